@@ -1,0 +1,200 @@
+// Backward of training-mode BatchNorm (+ ReLU, + residual input) from an 8-bit checkpoint of its input.
+//
+//   d       = dy where the layer's output was positive (the checkpoint's sign bits), else 0      (no ReLU: d = dy)
+//   dbeta_c = sum_r d,   dgamma_c = invstd_c * sum_r d (x8 - mean_c)
+//   dx      = gamma invstd (d - dbeta / R - xhat dgamma / R) = a d - b (x8 - mean) - c,   dres = d (+ racc)
+//
+// x8 is what the e4m3 codes stand for.  The sums need every row before the first dx, so dy and the codes are read twice: 2 x 3.16
+// bytes per bf16 element in, 2 (4 with a residual input) out.  A thread owns eight channels and walks rows, so the sums and the
+// coefficients stay in registers; partial sums are joined in a fixed order (results do not depend on the schedule).
+#include "mx_common.h"
+
+#define MXBN_MAX_GROUPS 1024
+
+struct MxBnGeom {
+    const void* dy;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const uint8_t* signs;      // nullptr: no ReLU
+    int64_t rows;
+    int C, cpr, blocks;        // cpr: 8-channel chunks per (padded) row of codes, blocks = cpr / 4
+    int lg;                    // log2 of the chunks a workgroup covers
+    int64_t per;               // rows per workgroup
+};
+
+// one row's d and x8 of a thread's chunk
+template <typename T, bool SIGNS>
+__device__ static inline void mxbn_load(const MxBnGeom& g, int64_t r, int c, int left, float (&d)[8], float (&v)[8]) {
+    const int64_t i = r * g.cpr + c;
+    const uint2 q = reinterpret_cast<const uint2*>(g.codes)[i];
+    const uint32_t b = g.scales[r * g.blocks + (c >> 2)];
+    mx_load8(reinterpret_cast<const T*>(g.dy) + r * g.C + c * 8, left, d);
+    if (SIGNS) {
+        const uint32_t m = g.signs[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = (m >> j) & 1 ? d[j] : 0.f;
+    }
+    mx_values_e4m3(q.x, q.y, mx_scale_value(b), v);
+}
+
+template <typename T, bool SIGNS>
+__global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const float* __restrict__ mean, float* __restrict__ part) {
+    __shared__ float red[4 * 32 * 16];
+    const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
+    const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
+    const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
+    float s0[8], s1[8], mu[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; mu[j] = j < left ? mean[c * 8 + j] : 0.f; }
+    if (left > 0) {
+#pragma unroll 4
+        for (int64_t r = r0 + rl; r < r1; r += nrl) {
+            float d[8], v[8];
+            mxbn_load<T, SIGNS>(g, r, c, left, d, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
+        }
+    }
+    // lanes of one chunk within the wave, then the four waves
+    for (int o = 32; o >= tc; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s0[j] += __shfl_xor(s0[j], o, 64); s1[j] += __shfl_xor(s1[j], o, 64); }
+    }
+    const int lane = tid & 63, wave = tid >> 6;
+    if (lane < tc) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { red[(wave * tc + lane) * 16 + j] = s0[j]; red[(wave * tc + lane) * 16 + 8 + j] = s1[j]; }
+    }
+    __syncthreads();
+    for (int t = tid; t < tc * 16; t += 256) {
+        const float s = (red[t] + red[tc * 16 + t]) + (red[2 * tc * 16 + t] + red[3 * tc * 16 + t]);
+        const int ch = (blockIdx.y * tc + (t >> 4)) * 8 + (t & 7);
+        if (ch < g.C) part[((int64_t)blockIdx.x * 2 + ((t >> 3) & 1)) * g.C + ch] = s;
+    }
+}
+
+// 32 channels x 8 partial rows per workgroup: totals, parameter gradients, and the coefficients a, b, c of dx
+__global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, float inv_rows,
+                                                           const float* __restrict__ gamma, const float* __restrict__ invstd,
+                                                           float* __restrict__ coef, float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                           int accumulate) {
+    __shared__ float red[2][8][32];
+    const int cl = threadIdx.x & 31, gl = threadIdx.x >> 5, ch = blockIdx.x * 32 + cl;
+    float s0 = 0.f, s1 = 0.f;
+    if (ch < C) {
+#pragma unroll 4
+        for (int g = gl; g < groups; g += 8) {
+            s0 += part[(int64_t)g * 2 * C + ch];
+            s1 += part[((int64_t)g * 2 + 1) * C + ch];
+        }
+    }
+    red[0][gl][cl] = s0;
+    red[1][gl][cl] = s1;
+    __syncthreads();
+    if (gl == 0 && ch < C) {
+        s0 = s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { s0 += red[0][k][cl]; s1 += red[1][k][cl]; }
+        const float is = invstd[ch], dg = s1 * is, a = gamma[ch] * is;
+        coef[ch] = a;
+        coef[C + ch] = a * is * dg * inv_rows;
+        coef[2 * C + ch] = a * s0 * inv_rows;
+        dgamma[ch] = accumulate ? dgamma[ch] + dg : dg;
+        dbeta[ch] = accumulate ? dbeta[ch] + s0 : s0;
+    }
+}
+
+template <typename T, bool SIGNS>
+__global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, const float* __restrict__ mean, const float* __restrict__ coef,
+                                                          T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc) {
+    const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
+    const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
+    if (left <= 0) return;
+    const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
+    float ka[8], kb[8], kc[8], mu[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int ch = c * 8 + j;
+        const bool ok = j < left;
+        ka[j] = ok ? coef[ch] : 0.f;
+        kb[j] = ok ? coef[g.C + ch] : 0.f;
+        kc[j] = ok ? coef[2 * g.C + ch] : 0.f;
+        mu[j] = ok ? mean[ch] : 0.f;
+    }
+#pragma unroll 4
+    for (int64_t r = r0 + rl; r < r1; r += nrl) {
+        float d[8], v[8], o[8];
+        mxbn_load<T, SIGNS>(g, r, c, left, d, v);
+        const int64_t at = r * g.C + c * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(ka[j], d[j], -fmaf(kb[j], v[j] - mu[j], kc[j]));
+        mx_store8(dx + at, left, o);
+        if (dres) {
+            if (racc) {
+                mx_load8(racc + at, left, o);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] += o[j];
+            }
+            mx_store8(dres + at, left, d);
+        }
+    }
+}
+
+static int mxbn_lg(int C) {
+    const int chunks = cdiv(C, 8);
+    int lg = 0;
+    while (lg < 5 && (1 << lg) < chunks) ++lg;
+    return lg;
+}
+// row groups of the sums pass: ~1024 workgroups in all, at least four rows for a thread
+static int mxbn_groups(int64_t rows, int C) {
+    const int lg = mxbn_lg(C), tiles = cdiv(cdiv(C, 8), 1 << lg);
+    const int64_t most = (rows + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
+    int64_t g = 1024 / tiles;
+    g = g < most ? g : most;
+    return (int)(g < 1 ? 1 : (g > MXBN_MAX_GROUPS ? MXBN_MAX_GROUPS : g));
+}
+
+extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C) {
+    if (rows < 1 || C < 1 || C > MX_MAX_C) return 0;
+    return sizeof(float) * ((size_t)mxbn_groups(rows, C) * 2 + 3) * (size_t)C;
+}
+
+extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scales, const void* signs, const float* gamma, const float* mean,
+                            const float* invstd, void* dx, void* dres, const void* racc, float* dgamma, float* dbeta, int accumulate,
+                            int64_t rows, int C, int dtype, void* ws, size_t ws_bytes, void* stream) {
+    CN_CHECK_ARG(rows >= 1 && C >= 1 && C <= MX_MAX_C && rows <= ((int64_t)1 << 40) / C, "cn_mx_bn_bwd: rows %lld, channels %d", (long long)rows, C);
+    CN_CHECK_ARG(dtype == CN_F32 || dtype == CN_BF16, "cn_mx_bn_bwd: bad dtype %d", dtype);
+    CN_CHECK_ARG(dy && codes && scales && gamma && mean && invstd && dx && dgamma && dbeta, "cn_mx_bn_bwd: null pointer");
+    CN_CHECK_ARG(dres || !racc, "cn_mx_bn_bwd: racc without dres");
+    CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_bn_bwd: codes must be 16-byte aligned");
+    if (!ws || ws_bytes < cn_mx_bn_bwd_bytes(rows, C)) {
+        cn_set_error("cn_mx_bn_bwd: workspace of %zu bytes needed", cn_mx_bn_bwd_bytes(rows, C));
+        return CN_EWORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const int groups = mxbn_groups(rows, C);
+    float* part = (float*)ws;
+    float* coef = part + (size_t)groups * 2 * C;
+    MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), mxbn_lg(C), 0};
+    const int tiles = cdiv(cdiv(C, 8), 1 << g.lg);
+    const int nrl = 256 >> g.lg;
+    CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
+    g.per = (rows + groups - 1) / groups;
+    CN_DISPATCH_DTYPE(dtype, T, {
+        if (signs) mx_bn_sums_kernel<T, true><<<dim3(groups, tiles), 256, 0, st>>>(g, mean, part);
+        else mx_bn_sums_kernel<T, false><<<dim3(groups, tiles), 256, 0, st>>>(g, mean, part);
+    });
+    CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    mx_bn_finish_kernel<<<cdiv(C, 32), 256, 0, st>>>(part, groups, C, 1.f / (float)rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
+    CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    g.per = 8 * nrl;
+    while ((rows + g.per - 1) / g.per > (int64_t)1 << 20) g.per *= 2;
+    const int ng = cdiv(rows, g.per);
+    CN_DISPATCH_DTYPE(dtype, T, {
+        if (signs) mx_bn_apply_kernel<T, true><<<dim3(ng, tiles), 256, 0, st>>>(g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
+        else mx_bn_apply_kernel<T, false><<<dim3(ng, tiles), 256, 0, st>>>(g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
+    });
+    CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    return CN_OK;
+}

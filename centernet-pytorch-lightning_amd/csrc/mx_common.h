@@ -1,0 +1,129 @@
+// Block-scaled ("MX") storage: up to 32 consecutive channels of a row share one power-of-two scale.
+//
+//   scale byte b: 2^(b - 127), 255 = not a number (the block held an infinity or a NaN: every value it stands for is a NaN)
+//   e4m3 codes: 1 byte, sign / 4 exponent / 3 significand bits, largest finite 448
+//   e2m1 codes: 4 bits (two to a byte, the even channel in the low half), values 0 .5 1 1.5 2 3 4 6
+//   codes [rows][Cp * bits / 8] with Cp = C rounded up to 32 (the filler stands for zeros), scales [rows][Cp / 32],
+//   sign bits (optional) [rows][Cp / 8]: bit j of byte i = (source[8 i + j] > 0)
+#pragma once
+#include "common.h"
+
+#define MX_BLOCK 32
+#define MX_MAX_C 65536            // chunk arithmetic below stays in 32 bits
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+// 16 bytes at any 2- / 4-byte aligned address: rows of an odd number of channels start anywhere, and the hardware loads and stores
+// such vectors in one instruction all the same
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Exponent byte of a block's scale from the bits of its largest magnitude a (as float): the least power of two for which a / scale
+// rounds to a finite element.  The elements' top binade ends where rounding would carry past the largest one — at 1.75 * 2^emax for
+// e2m1 (the tie 7 would go to 8), just above 1.8125 * 2^emax for e4m3 (the tie 464 goes to 448) — so adding the distance from there to
+// 2 makes the significand carry into the exponent exactly when the next scale is needed.
+template <int FMT> __device__ static inline uint32_t mx_scale_byte(uint32_t abs_bits) {
+    constexpr uint32_t carry = FMT == CN_MX_E2M1 ? 0x200000u : 0x17ffffu;
+    constexpr int emax = FMT == CN_MX_E2M1 ? 2 : 8;
+    const int e = (int)((abs_bits + carry) >> 23) - emax;
+    return abs_bits >= 0x7f800000u ? 255u : (uint32_t)(e > 0 ? e : 0);
+}
+// 2^(b - 127) as float (b = 0: subnormal; 255: NaN)
+__device__ static inline float mx_scale_value(uint32_t b) {
+    return __uint_as_float(b == 255u ? 0x7fc00000u : (b == 0u ? 0x00400000u : b << 23));
+}
+// 2^(127 - b) for a finite scale byte (b <= 253 by construction: normal)
+__device__ static inline float mx_scale_inverse(uint32_t b) { return __uint_as_float((254u - b) << 23); }
+
+// bitwise maximum over the four lanes of a quad
+__device__ static inline uint32_t quad_max_u(uint32_t v) {
+    const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);      // quad_perm [1,0,3,2]
+    v = a > v ? a : v;
+    const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);      // quad_perm [2,3,0,1]
+    return b > v ? b : v;
+}
+
+// eight consecutive elements of a row as floats, zero behind the row's end (`left` = channels from here to the end, may be <= 0)
+__device__ static inline void mx_load8(const float* p, int left, float (&v)[8]) {
+    if (left >= 8) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_a4*>(p), b = *reinterpret_cast<const u32x4_a4*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+    }
+}
+__device__ static inline void mx_load8(const bf16_t* p, int left, float (&v)[8]) {
+    if (left >= 8) {
+        const u32x4_t a = *reinterpret_cast<const u32x4_a2*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(a[i] << 16); v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? bf2f(p[i]) : 0.f;
+    }
+}
+__device__ static inline void mx_store8(float* p, int left, const float (&v)[8]) {
+    if (left >= 8) {
+        *reinterpret_cast<u32x4_a4*>(p) = u32x4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        *reinterpret_cast<u32x4_a4*>(p + 4) = u32x4_t{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < left) p[i] = v[i];
+    }
+}
+__device__ static inline void mx_store8(bf16_t* p, int left, const float (&v)[8]) {
+    if (left >= 8) {
+        *reinterpret_cast<u32x4_a2*>(p) = u32x4_t{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) if (i < left) p[i] = f2bf(v[i]);
+    }
+}
+
+__device__ static inline uint32_t mx_absmax8(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; m = a > m ? a : m; }
+    return m;
+}
+// codes of eight values on scale byte b (255: zeros); e2m1 -> 4 bytes, e4m3 -> 8 bytes.  Both conversions round to nearest even, and
+// the scale is an exact power of two: one rounding in all.
+__device__ static inline uint32_t mx_codes_e2m1(const float (&v)[8], uint32_t b) {
+    const float s = mx_scale_value(b);
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
+    return b == 255u ? 0u : r;
+}
+__device__ static inline uint2 mx_codes_e4m3(const float (&v)[8], uint32_t b) {
+    const float s = b == 255u ? 0.f : mx_scale_inverse(b);
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * s, v[1] * s, lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * s, v[3] * s, lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * s, v[5] * s, hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * s, v[7] * s, hi, true);
+    return b == 255u ? make_uint2(0u, 0u) : make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+// the eight values that 8 bytes of e4m3 codes stand for
+__device__ static inline void mx_values_e4m3(uint32_t lo, uint32_t hi, float s, float (&v)[8]) {
+    f32x2_t p = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false); v[0] = p.x * s; v[1] = p.y * s;
+    p = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);          v[2] = p.x * s; v[3] = p.y * s;
+    p = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false);         v[4] = p.x * s; v[5] = p.y * s;
+    p = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);          v[6] = p.x * s; v[7] = p.y * s;
+}
+__device__ static inline void mx_values_e2m1(uint32_t c, float s, float (&v)[8]) {
+    f32x2_t p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0); v[0] = p.x * s; v[1] = p.y * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);         v[2] = p.x * s; v[3] = p.y * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);         v[4] = p.x * s; v[5] = p.y * s;
+    p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);         v[6] = p.x * s; v[7] = p.y * s;
+}
+
+// n / d for n * d < 2^32 by one high multiplication (m = ceil(2^32 / d); d = 1 has m = 0)
+struct MxDiv { uint32_t d, m; };
+static inline MxDiv mx_div(uint32_t d) { return MxDiv{d, d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)}; }
+__device__ static inline uint32_t mx_quot(uint32_t n, MxDiv v) { return v.m ? __umulhi(n, v.m) : n; }

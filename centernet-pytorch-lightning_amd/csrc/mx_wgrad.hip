@@ -1,0 +1,317 @@
+// Weight (and bias) gradient of a linear layer / 1x1 convolution from an 8-bit checkpoint of its input:
+//   dw[n][k] = sum_r dy[r][n] * x8[r][k],   db[n] = sum_r dy[r][n]
+//
+// The sum runs over rows, the slow axis of both operands.  Tiles are staged in their natural [row][channel] order — the e4m3 codes
+// become bf16 on the way (exact: four significant bits times a power of two) — and the transposing LDS read hands every lane eight
+// rows of its channel (rows padded by 64 B: the four rows of a read hit disjoint banks).  A 32-bit dy is split into three bf16 terms
+// (8 + 8 + 8 significant bits: nothing is lost) that share the x8 fragment.
+// Row ranges are split over workgroups; their partial sums go to the workspace and are added in a fixed order.
+#include "mx_common.h"
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+
+// 32(channel) x 16(row) operand out of a [row][channel] LDS tile: lane l gets channel r0 + (l & 31), rows k0 + 8 * (l >> 5) .. + 7
+__device__ static inline bf16x8_t mx_tr_frag(const bf16_t* tile, int pitch, int r0, int k0, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    const bf16_t* p = tile + (k0 + 8 * (g >> 1) + (r >> 2)) * pitch + r0 + 16 * (g & 1) + 4 * (r & 3);
+    typedef __attribute__((address_space(3))) s16x4_t* lds_ptr;
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * pitch));
+    const s16x8_t v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(bf16x8_t, v);
+}
+
+struct MxWgGeom {
+    const void* dy;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    float* dw;                 // [splits][N][K] partial sums, or the gradient itself (splits == 1)
+    float* db;                 // [splits][N], or the gradient itself; nullptr: none
+    int64_t rows, per;         // per: rows of one split (a multiple of the row tile)
+    int N, K, Kp, blocks;
+    int ktiles, accumulate;
+};
+
+// Eight raw dy elements; FULL: N is a multiple of 8, a chunk is inside the row or outside (branch-free: a readable address, masked)
+template <typename T> struct MxRaw8;
+template <> struct MxRaw8<bf16_t> {
+    uint4 a;
+    template <bool FULL> __device__ inline void load(const bf16_t* base, int64_t at, int left, bool ok) {
+        if (FULL) {
+            ok = ok && left > 0;
+            const u32x4_t v = *reinterpret_cast<const u32x4_a2*>(base + (ok ? at : 0));
+            const uint32_t m = ok ? 0xffffffffu : 0u;
+            a = make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
+        } else {
+            float f[8];
+            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
+            a = make_uint4(pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7]));
+        }
+    }
+    __device__ inline void get(float (&f)[8]) const { Vec16<bf16_t>::unpack(a, f); }
+    __device__ inline void put(bf16_t* lds, int) const { st16(lds, a); }
+};
+template <> struct MxRaw8<float> {
+    float f[8];
+    template <bool FULL> __device__ inline void load(const float* base, int64_t at, int left, bool ok) {
+        if (FULL) {
+            ok = ok && left > 0;
+            const float* p = base + (ok ? at : 0);
+            const u32x4_t v = *reinterpret_cast<const u32x4_a4*>(p), w = *reinterpret_cast<const u32x4_a4*>(p + 4);
+            const uint32_t m = ok ? 0xffffffffu : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(v[i] & m); f[4 + i] = __uint_as_float(w[i] & m); }
+        } else {
+            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
+        }
+    }
+    __device__ inline void get(float (&o)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = f[i];
+    }
+    // three planes, `plane` elements apart: truncation to 8 significant bits twice, the rest is exact; an infinity or NaN is all in the first
+    __device__ inline void put(bf16_t* lds, int plane) const {
+        uint32_t h[8], m[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t u = __float_as_uint(f[i]);
+            const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+            h[i] = fin ? u & 0xffff0000u : ((u & 0x7fffffu) ? 0x7fc00000u : u);
+            const float r = fin ? f[i] - __uint_as_float(h[i]) : 0.f;
+            m[i] = __float_as_uint(r) & 0xffff0000u;
+            l[i] = __float_as_uint(r - __uint_as_float(m[i]));
+        }
+#define MX_PK(x) make_uint4((x[0] >> 16) | (x[1] & 0xffff0000u), (x[2] >> 16) | (x[3] & 0xffff0000u), (x[4] >> 16) | (x[5] & 0xffff0000u), (x[6] >> 16) | (x[7] & 0xffff0000u))
+        st16(lds, MX_PK(h));
+        st16(lds + plane, MX_PK(m));
+        st16(lds + 2 * plane, MX_PK(l));
+#undef MX_PK
+    }
+};
+
+template <typename T, int TN, int TK, bool FULL>
+__global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
+    constexpr int NP = sizeof(T) == 2 ? 1 : 3;
+    constexpr int BR = 64;                                        // rows per tile
+    constexpr int YP = TN + 32, XP = TK + 32;                     // LDS pitches (elements)
+    constexpr int YV = BR * TN / 8 / 256, XV = BR * TK / 16 / 256;
+    constexpr int YC = TN / 8, XC = TK / 16;
+    constexpr int MI = TN / 64, NJ = TK / 64;                     // 2 x 2 waves of 32 x 32 tiles
+    constexpr int PLANE = BR * YP;
+    __shared__ __attribute__((aligned(16))) bf16_t lds[NP * PLANE + BR * XP];
+    bf16_t* const ly = lds;
+    bf16_t* const lx = lds + NP * PLANE;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave >> 1, wn = wave & 1;
+    const int nt = blockIdx.y / g.ktiles, kt = blockIdx.y - nt * g.ktiles;
+    const int n0 = nt * TN, k0 = kt * TK;
+    const int64_t rbeg = (int64_t)blockIdx.x * g.per, rend = rbeg + g.per < g.rows ? rbeg + g.per : g.rows;
+    const bool bias = g.db != nullptr && kt == 0;
+
+    const int yc = (tid % YC) * 8, yr = tid / YC;                 // dy: chunk column (the same for all YV loads), first row
+    const int xc = (tid % XC) * 16, xr = tid / XC;
+    const int yleft = g.N - n0 - yc;
+    const bool xok = k0 + xc < g.Kp;                              // (Kp is a multiple of 32: 16 codes are inside or outside)
+
+    MxRaw8<T> ry[YV];
+    uint4 rx[XV];
+    uint32_t rs[XV];
+    auto gload = [&](int64_t r0) {
+#pragma unroll
+        for (int v = 0; v < YV; ++v) {
+            const int64_t r = r0 + yr + v * (256 / YC);
+            ry[v].template load<FULL>(reinterpret_cast<const T*>(g.dy), r * g.N + n0 + yc, yleft, r < rend);
+        }
+#pragma unroll
+        for (int v = 0; v < XV; ++v) {
+            const int64_t r = r0 + xr + v * (256 / XC);
+            const bool ok = xok && r < rend;
+            rx[v] = ldg16_masked(g.codes, r * g.Kp + k0 + xc, ok);
+            rs[v] = g.scales[ok ? r * g.blocks + ((k0 + xc) >> 5) : 0];
+            rs[v] = ok ? rs[v] : 127u;                            // (codes are zero there: any finite scale)
+        }
+    };
+    float sb[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sb[j] = 0.f;
+    auto lstore = [&]() {
+#pragma unroll
+        for (int v = 0; v < YV; ++v) {
+            ry[v].put(ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
+            if (bias) {
+                float f[8];
+                ry[v].get(f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sb[j] += f[j];
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < XV; ++v) {
+            const float s = mx_scale_value(rs[v]);
+            const uint32_t w[4] = {rx[v].x, rx[v].y, rx[v].z, rx[v].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, false));
+                o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, true));
+            }
+            bf16_t* p = lx + (xr + v * (256 / XC)) * XP + xc;
+            st16(p, make_uint4(o[0], o[1], o[2], o[3]));
+            st16(p + 8, make_uint4(o[4], o[5], o[6], o[7]));
+        }
+    };
+
+    f32x16_t acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+    gload(rbeg);
+    for (int64_t r0 = rbeg; r0 < rend; r0 += BR) {
+        __syncthreads();                                          // the previous tile has been read
+        lstore();
+        __syncthreads();
+        if (r0 + BR < rend) gload(r0 + BR);
+#pragma unroll
+        for (int s = 0; s < BR / 16; ++s) {
+            bf16x8_t b[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) b[j] = mx_tr_frag(lx, XP, (wn * NJ + j) * 32, s * 16, lane);
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    const bf16x8_t a = mx_tr_frag(ly + p * PLANE, YP, (wm * MI + i) * 32, s * 16, lane);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+                }
+        }
+    }
+
+    float* dw = g.dw + (int64_t)blockIdx.x * g.N * g.K;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int k = k0 + (wn * NJ + j) * 32 + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int n = n0 + (wm * MI + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                if (n < g.N && k < g.K) {
+                    float* p = dw + (int64_t)n * g.K + k;
+                    *p = g.accumulate ? *p + acc[i][j][e] : acc[i][j][e];
+                }
+            }
+        }
+    if (bias) {
+        float* red = reinterpret_cast<float*>(lds);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) red[tid * 8 + j] = sb[j];
+        __syncthreads();
+        if (tid < TN) {
+            float s = 0.f;
+            for (int q = 0; q < 256 / YC; ++q) s += red[(q * YC + (tid >> 3)) * 8 + (tid & 7)];
+            float* p = g.db + (int64_t)blockIdx.x * g.N + n0 + tid;
+            if (n0 + tid < g.N) *p = g.accumulate ? *p + s : s;
+        }
+    }
+}
+
+// out[i] = (accumulate ? out[i] : 0) + sum_s part[s][i], the splits in order
+__global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int splits,
+                                                            const float* __restrict__ part_b, float* __restrict__ out_b, int nb, int accumulate) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n + nb) return;
+    const bool w = i < n;
+    const float* p = w ? part + i : part_b + (i - n);
+    const int64_t step = w ? n : nb;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += p[(int64_t)k * step];
+    float* o = w ? out + i : out_b + (i - n);
+    *o = accumulate ? *o + s : s;
+}
+
+struct MxWgPlan { int tn, tk, ntiles, ktiles, splits; int64_t per; };
+static MxWgPlan mxwg_plan(int64_t rows, int K, int N, int dtype) {
+    MxWgPlan p;
+    p.tn = (N > 64 && dtype == CN_BF16) ? 128 : 64;
+    p.tk = K > 64 ? 128 : 64;
+    p.ntiles = cdiv(N, p.tn);
+    p.ktiles = cdiv(K, p.tk);
+    const int64_t tiles = (int64_t)p.ntiles * p.ktiles, rtiles = (rows + 63) / 64;
+    int64_t s = 768 / tiles;                      // three workgroups a CU
+    s = s < rtiles ? s : rtiles;
+    s = s < 1 ? 1 : s;
+    p.per = (rtiles + s - 1) / s * 64;
+    p.splits = (int)((rows + p.per - 1) / p.per);
+    return p;
+}
+
+extern "C" size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype) {
+    if (rows < 1 || K < 1 || N < 1 || K > MX_MAX_C || N > MX_MAX_C) return 0;
+    const MxWgPlan p = mxwg_plan(rows, K, N, dtype);
+    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * ((size_t)N * K + N) : 16;
+}
+
+template <typename T, int TN, int TK>
+static void mxwg_launch(const MxWgGeom& g, const MxWgPlan& p, hipStream_t st) {
+    const dim3 grid(p.splits, p.ntiles * p.ktiles);
+    if (g.N % 8 == 0) mx_wgrad_kernel<T, TN, TK, true><<<grid, 256, 0, st>>>(g);
+    else mx_wgrad_kernel<T, TN, TK, false><<<grid, 256, 0, st>>>(g);
+}
+
+extern "C" int cn_mx_linear_wgrad(const void* dy, const void* codes, const void* scales, float* dw, float* db, int accumulate, int64_t rows,
+                                  int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream) {
+    CN_CHECK_ARG(rows >= 1 && K >= 1 && N >= 1 && K <= MX_MAX_C && N <= MX_MAX_C && rows <= ((int64_t)1 << 40) / (K > N ? K : N),
+                 "cn_mx_linear_wgrad: rows %lld, K %d, N %d", (long long)rows, K, N);
+    CN_CHECK_ARG(dtype == CN_F32 || dtype == CN_BF16, "cn_mx_linear_wgrad: bad dtype %d", dtype);
+    CN_CHECK_ARG(dy && codes && scales && dw, "cn_mx_linear_wgrad: null pointer");
+    CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_linear_wgrad: codes must be 16-byte aligned");
+    if (!ws || ws_bytes < cn_mx_linear_wgrad_bytes(rows, K, N, dtype)) {
+        cn_set_error("cn_mx_linear_wgrad: workspace of %zu bytes needed", cn_mx_linear_wgrad_bytes(rows, K, N, dtype));
+        return CN_EWORKSPACE;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    const MxWgPlan p = mxwg_plan(rows, K, N, dtype);
+    CN_CHECK_ARG((int64_t)p.ntiles * p.ktiles <= 65535, "cn_mx_linear_wgrad: K x N too large");
+    const bool join = p.splits > 1;
+    MxWgGeom g;
+    g.dy = dy;
+    g.codes = (const uint8_t*)codes;
+    g.scales = (const uint8_t*)scales;
+    g.dw = join ? (float*)ws : dw;
+    g.db = db ? (join ? (float*)ws + (size_t)p.splits * N * K : db) : nullptr;
+    g.rows = rows;
+    g.per = p.per;
+    g.N = N;
+    g.K = K;
+    g.blocks = cdiv(K, MX_BLOCK);
+    g.Kp = g.blocks * MX_BLOCK;
+    g.ktiles = p.ktiles;
+    g.accumulate = join ? 0 : accumulate;
+    if (dtype == CN_BF16) {
+        if (p.tn == 128 && p.tk == 128) mxwg_launch<bf16_t, 128, 128>(g, p, st);
+        else if (p.tn == 128) mxwg_launch<bf16_t, 128, 64>(g, p, st);
+        else if (p.tk == 128) mxwg_launch<bf16_t, 64, 128>(g, p, st);
+        else mxwg_launch<bf16_t, 64, 64>(g, p, st);
+    } else {
+        if (p.tk == 128) mxwg_launch<float, 64, 128>(g, p, st);
+        else mxwg_launch<float, 64, 64>(g, p, st);
+    }
+    CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
+    if (join) {
+        const int64_t n = (int64_t)N * K;
+        const int nb = db ? N : 0;
+        mx_wgrad_join_kernel<<<(unsigned)((n + nb + 255) / 256), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
+    }
+    return CN_OK;
+}

@@ -24,6 +24,10 @@ extern "C" {
 #define CN_F32 0
 #define CN_BF16 1
 
+/* element formats of the block-scaled ("MX") operators */
+#define CN_MX_E2M1 0 /* 4 bits */
+#define CN_MX_E4M3 1 /* 8 bits */
+
 #define CN_OK 0
 #define CN_EINVAL (-1)
 #define CN_EUNSUPPORTED (-2)
@@ -533,6 +537,35 @@ int cn_adam_step(float* p, const float* g, float* m, float* v, int64_t n, float 
  * t as int32 bits}.  Launched right before cn_adam_step (inside the same captured graph), so replays never depend on a
  * per-step host upload; the host only writes hyper[0] when the learning rate changes and hyper[3] when it restores t. */
 int cn_adam_advance(float* hyper, float b1, float b2, void* stream);
+
+/* ---- block-scaled 8- / 4-bit floating point: storage, 4-bit product, backward passes from 8-bit activation checkpoints ----
+ * Up to 32 consecutive channels of a row share one scale 2^(byte - 127): the least power of two for which no element of the block
+ * rounds past the largest finite one (448 for e4m3, 6 for e2m1); byte 255: the block held an infinity or a NaN, all its values are NaN.
+ * Values are rounded to nearest even.  With Cp = C rounded up to 32:
+ *   codes  [rows][Cp] bytes (CN_MX_E4M3) or [rows][Cp / 2] (CN_MX_E2M1, even channel in the low half), 16-byte aligned, filler 0
+ *   scales [rows][Cp / 32] bytes;  signs [rows][Cp / 8] bytes, bit j of byte i = (sign_src[8 i + j] > 0)
+ * 1 <= C <= 65536; rows of x may start at any element-aligned address. */
+/* sign_src / signs: both or neither (what a ReLU's backward pass needs to know of its output, 1 bit) */
+int cn_mx_quantize(const void* x, void* codes, void* scales, const void* sign_src, void* signs, int64_t rows, int C, int fmt,
+                   int dtype, void* stream);
+int cn_mx_dequantize(const void* codes, const void* scales, void* out, int64_t rows, int C, int fmt, int dtype, void* stream);
+/* weights w [N][K] -> e2m1 codes and scales in the product's fragment order (cn_mx_weight_bytes bytes, 16-byte aligned) */
+size_t cn_mx_weight_bytes(int N, int K);
+int cn_mx_pack_weight(const void* w, void* packed, int N, int K, int dtype, void* stream);
+/* y [M][N] = act(e2m1(x [M][K]) @ w4^T + bias + residual); x, residual and y in `dtype`, bias fp32 [N] */
+int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const void* residual, void* y, int64_t M, int K, int N,
+                     int relu, int dtype, void* stream);
+/* dw [N][K] (+)= dy^T @ x8, db [N] (+)= column sums of dy (db may be null); x8 = e4m3 checkpoint [rows][K], dy [rows][N] in `dtype`.
+ * Sums in a fixed order: the same inputs give the same bits. */
+size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype);
+int cn_mx_linear_wgrad(const void* dy, const void* codes, const void* scales, float* dw, float* db, int accumulate, int64_t rows,
+                       int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream);
+/* backward of y = [relu](gamma * (x - mean) * invstd + beta [+ residual]) with batch statistics, from an e4m3 checkpoint of x; signs:
+ * the ReLU's sign bits (null: no ReLU).  dres (may be null): gradient of the residual input, plus racc (may be null). */
+size_t cn_mx_bn_bwd_bytes(int64_t rows, int C);
+int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scales, const void* signs, const float* gamma, const float* mean,
+                 const float* invstd, void* dx, void* dres, const void* racc, float* dgamma, float* dbeta, int accumulate,
+                 int64_t rows, int C, int dtype, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
