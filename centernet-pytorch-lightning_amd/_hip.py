@@ -156,6 +156,28 @@ def try_call(name, *args, hooks=None):
     return True
 
 
+_entries = {}
+
+
+def launch(name, device, *args):
+    """`call` without its per-argument conversions, for entry points whose work is shorter than those: `args` are ready (integers, and
+    pointers as integers or None), the stream is the current one of CUDA device index `device`, which may differ from the current device."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(lib(), name)
+    if TRACE:
+        import sys
+        sys.stderr.write(f"CALL {name} {args}\n")
+        sys.stderr.flush()
+    if device == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        raise RuntimeError(f"{name} failed (status {rc}): {lib().cn_last_error().decode()}")
+
+
 def query(name, *args):
     """size_t / int queries without a stream argument."""
     return getattr(lib(), name)(*args)

@@ -83,6 +83,58 @@ __device__ static inline void mx_store8(bf16_t* p, int left, const float (&v)[8]
     }
 }
 
+// Eight consecutive elements as they lie in memory, so that several loads can be in flight before the first is unpacked.  FULL: the row
+// has a multiple of 8 channels, so a chunk lies inside it or outside (branch-free: a readable address, masked; an exec-masked branch
+// would make the compiler wait for every load before the next); otherwise the row's last chunk is read element by element.
+template <typename T> struct MxRaw8;
+template <> struct MxRaw8<bf16_t> {
+    u32x4_t a;
+    template <bool FULL> __device__ inline void load(const bf16_t* base, int64_t at, int left, bool ok) {
+        if (FULL) {
+            ok = ok && left > 0;
+            const u32x4_t v = *reinterpret_cast<const u32x4_a2*>(base + (ok ? at : 0));
+            const uint32_t m = ok ? 0xffffffffu : 0u;
+            a = u32x4_t{v.x & m, v.y & m, v.z & m, v.w & m};
+        } else {
+            float f[8];
+            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
+            a = u32x4_t{pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7])};
+        }
+    }
+    __device__ inline void get(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(a[i] << 16); f[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+    }
+};
+template <> struct MxRaw8<float> {
+    u32x4_t a, b;
+    template <bool FULL> __device__ inline void load(const float* base, int64_t at, int left, bool ok) {
+        if (FULL) {
+            ok = ok && left > 0;
+            const float* p = base + (ok ? at : 0);
+            const u32x4_t v = *reinterpret_cast<const u32x4_a4*>(p), w = *reinterpret_cast<const u32x4_a4*>(p + 4);
+            const uint32_t m = ok ? 0xffffffffu : 0u;
+            a = u32x4_t{v.x & m, v.y & m, v.z & m, v.w & m};
+            b = u32x4_t{w.x & m, w.y & m, w.z & m, w.w & m};
+        } else {
+            float f[8];
+            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { a[i] = __float_as_uint(f[i]); b[i] = __float_as_uint(f[4 + i]); }
+        }
+    }
+    __device__ inline void get(float (&f)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(a[i]); f[4 + i] = __uint_as_float(b[i]); }
+    }
+};
+
+// store of eight elements of such a row (FULL as above)
+template <bool FULL, typename T> __device__ static inline void mx_store8f(T* p, int left, const float (&v)[8]) {
+    if (FULL) { if (left > 0) mx_store8(p, 8, v); }
+    else mx_store8(p, left, v);
+}
+
 __device__ static inline uint32_t mx_absmax8(const float (&v)[8]) {
     uint32_t m = 0;
 #pragma unroll

@@ -66,33 +66,38 @@ struct MxLinGeom {
     const void* res;
     void* y;
     int64_t M;
-    int K, N, S, S4;           // S: steps of 64 channels, S4 = ceil(S / 4)
+    int K, N, S, S4;           // S: steps of 64 channels, S4 = ceil(S / 4) groups
+    int t32;                   // 32-column tiles in all
     int chunk;                 // steps that LDS holds (a multiple of 4 unless it is S)
-    int ntiles;                // 64-column tiles in all
-    int per_wg;                // passes over the waves' columns per workgroup
+    int per_wg;                // passes over the workgroup's columns
     int relu;
     int pitch, spitch;         // LDS bytes per row: codes, scales
-    MxDiv cdiv_full, cdiv_last;        // 8-channel pieces per row of a full / the last chunk
+    MxDiv div_full, div_last;  // 8-channel pieces per row of a full / the last chunk
     int sc_ofs, ep_ofs;        // LDS offsets of the scales and of the output staging
 };
 
-#define MXL_EP 68              // floats per staged output row (64 + 4: rows on different banks)
+// two steps of NJ weight tiles
+template <int NJ> struct MxLinB { u32x4_t f[2][NJ]; };
 
-template <typename T, int BM, int WM>
-__global__ __launch_bounds__(256) void mx_linear_kernel(const MxLinGeom g) {
-    constexpr int WN = 4 / WM, MI = BM / WM / 32;
+// MI x NJ tiles of 32 x 32 per wave; WM x WN waves over rows and columns, WK over the channels (few rows: the launch would be short of
+// waves otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows
+template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULL, bool resident>
+__global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
+    static_assert(WM * WN * WK == 4 && (WK == 1 || (WK == 4 && MI == 1)), "four waves");
+    constexpr int BM = 32 * MI * WM, EPN = 32 * NJ, EPP = EPN + 4;         // EPP: floats per staged output row (rows on different banks)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = WK > 1 ? 0 : wave / WN, wn = WK > 1 ? 0 : wave % WN, wk = WK > 1 ? wave : 0;
     const int64_t m0 = (int64_t)blockIdx.x * BM;
     const int rows = (int)(g.M - m0 < BM ? g.M - m0 : BM);
     const T* __restrict__ X = reinterpret_cast<const T*>(g.x) + m0 * g.K;
 
-    auto stage = [&](int s0, int s1) {                            // quantise channels 64 s0 .. 64 s1 of the workgroup's rows into LDS
-        const MxDiv dv = s1 == g.S ? g.cdiv_last : g.cdiv_full;
-        const int total = BM * (int)dv.d;
-        constexpr int U = 4;
+    // quantise channels 64 s0 .. 64 s1 of the workgroup's rows into LDS (rows behind the last stay as they are: what they give is not stored)
+    auto stage = [&](int s0, int s1) {
+        const MxDiv dv = s1 == g.S ? g.div_last : g.div_full;
+        const int total = rows * (int)dv.d;
+        constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;            // loads in flight per thread
         for (int base = tid; base < total; base += 256 * U) {
-            float v[U][8];
+            MxRaw8<T> v[U];
             int row[U], pc[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -100,159 +105,233 @@ __global__ __launch_bounds__(256) void mx_linear_kernel(const MxLinGeom g) {
                 row[u] = (int)mx_quot(i, dv);
                 pc[u] = (int)i - row[u] * (int)dv.d;
                 const int c0 = s0 * 64 + pc[u] * 8;
-                mx_load8(X + (int64_t)row[u] * g.K + c0, ((int)i < total && row[u] < rows) ? g.K - c0 : 0, v[u]);
+                v[u].template load<FULL>(X, (int64_t)row[u] * g.K + c0, g.K - c0, (int)i < total);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(mx_absmax8(v[u])));
+                float f[8];
+                v[u].get(f);
+                const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(mx_absmax8(f)));
                 if (base + u * 256 < total) {                     // (whole quads)
-                    *reinterpret_cast<uint32_t*>(smem + row[u] * g.pitch + pc[u] * 4) = mx_codes_e2m1(v[u], b);
+                    *reinterpret_cast<uint32_t*>(smem + row[u] * g.pitch + pc[u] * 4) = mx_codes_e2m1(f, b);
                     const int blk = pc[u] >> 2, s = blk >> 1;     // byte s & 3 of word (s / 4, half)
                     if ((pc[u] & 3) == 0) smem[g.sc_ofs + row[u] * g.spitch + ((s >> 2) * 2 + (blk & 1)) * 4 + (s & 3)] = (uint8_t)b;
                 }
             }
         }
     };
-
-    const bool resident = g.chunk >= g.S;
-    if (resident) { stage(0, g.S); __syncthreads(); }
-
+    // steps s, s + 1 and the scales of their group for the columns of pass `it` (beyond the last: a readable address, not used)
+    auto loadb = [&](MxLinB<NJ>& B, int it, int s) {
+        const int first = ((blockIdx.y * g.per_wg + it) * WN + wn) * NJ;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int nt = first + j < g.t32 ? first + j : g.t32 - 1;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int q = s + u < g.S ? s + u : g.S - 1;
+                // (a uniform base and a lane offset: no address registers; the index stays below 2^28)
+                B.f[u][j] = reinterpret_cast<const u32x4_t*>(g.wc + __builtin_amdgcn_readfirstlane((nt * g.S + q) * 64))[lane];
+            }
+        }
+    };
+    auto loads = [&](uint32_t (&q)[NJ], int it, int t) {
+        const int first = ((blockIdx.y * g.per_wg + it) * WN + wn) * NJ;
+        t = t < g.S4 ? t : g.S4 - 1;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) q[j] = (g.ws + __builtin_amdgcn_readfirstlane(((first + j < g.t32 ? first + j : g.t32 - 1) * g.S4 + t) * 64))[lane];
+    };
+    f32x16_t acc[MI][NJ];
     const unsigned char* arow = smem + (wm * MI * 32 + (lane & 31)) * g.pitch + (lane >> 5) * 16;
     const unsigned char* srow = smem + g.sc_ofs + (wm * MI * 32 + (lane & 31)) * g.spitch + (lane >> 5) * 4;
-    float* ep = reinterpret_cast<float*>(smem + g.ep_ofs) + wave * 32 * MXL_EP;
-
-    for (int it = 0; it < g.per_wg; ++it) {
-        const int tile = (blockIdx.y * g.per_wg + it) * WN + wn;  // 64 columns
-        const bool live = tile < g.ntiles;
-        if (resident && !live) break;                             // (no barrier below in the resident form)
-        const int t32 = (g.N + 31) >> 5, nt0 = live ? tile * 2 : 0, nt1 = nt0 + 1 < t32 ? nt0 + 1 : nt0;   // (an odd count: the last tile twice)
-        f32x16_t acc[MI][2];
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-        for (int s0 = 0; s0 < g.S; s0 += g.chunk) {
-            const int s1 = s0 + g.chunk < g.S ? s0 + g.chunk : g.S;
-            if (!resident) {
-                __syncthreads();
-                stage(s0, s1);
-                __syncthreads();
-            }
-            const uint4* b0 = g.wc + (int64_t)nt0 * g.S * 64 + lane;
-            const uint4* b1 = g.wc + (int64_t)nt1 * g.S * 64 + lane;
-            const uint32_t* q0 = g.ws + (int64_t)nt0 * g.S4 * 64 + lane;
-            const uint32_t* q1 = g.ws + (int64_t)nt1 * g.S4 * 64 + lane;
-            for (int t = s0 >> 2; 4 * t < s1; ++t) {
-                const uint32_t sb0 = q0[t * 64], sb1 = q1[t * 64];
-                uint32_t sa[MI];
-#pragma unroll
-                for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(srow + i * 32 * g.spitch + (t - (s0 >> 2)) * 8);
-                uint4 fb[4][2];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int s = 4 * t + u < s1 ? 4 * t + u : s1 - 1;
-                    fb[u][0] = ldg16(b0 + s * 64);
-                    fb[u][1] = ldg16(b1 + s * 64);
-                }
-#define MXL_STEP(u)                                                                                                                     \
-    if (4 * t + u < s1) {                                                                                                               \
+    // steps s (with byte U of the scale words) and s + 1
+#define MXL_STEP(B, u, U)                                                                                                               \
+    if (s + u < s1) {                                                                                                                   \
         _Pragma("unroll") for (int i = 0; i < MI; ++i) {                                                                                \
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(arow + i * 32 * g.pitch + (4 * t + u - s0) * 32);                       \
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(arow + i * 32 * g.pitch + (s + u - s0) * 32);                           \
             const i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};                                                    \
-            _Pragma("unroll") for (int j = 0; j < 2; ++j) {                                                                             \
-                const i32x8_t bv = {(int)fb[u][j].x, (int)fb[u][j].y, (int)fb[u][j].z, (int)fb[u][j].w, 0, 0, 0, 0};                    \
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 4, 4, u, (int)sa[i], u, (int)(j ? sb1 : sb0)); \
+            _Pragma("unroll") for (int j = 0; j < NJ; ++j) {                                                                            \
+                const i32x8_t bv = {(int)B.f[u][j].x, (int)B.f[u][j].y, (int)B.f[u][j].z, (int)B.f[u][j].w, 0, 0, 0, 0};                \
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 4, 4, U, (int)sa[i], U, (int)sb[j]);     \
             }                                                                                                                           \
         }                                                                                                                               \
     }
-                MXL_STEP(0) MXL_STEP(1) MXL_STEP(2) MXL_STEP(3)
-#undef MXL_STEP
+    // eight finished columns of a row; rv: the residual input there (zeros: none)
+    auto finish = [&](float (&v)[8], const MxRaw8<T>& rv, int64_t m, int nc, int left, const float (&bs)[8]) {
+        float r[8];
+        rv.get(r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += bs[e];
+        if (g.res) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+        }
+        if (g.relu) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];            // (a NaN stays one)
+        }
+        if (m < g.M) mx_store8f<FULL>(reinterpret_cast<T*>(g.y) + m * g.N + nc, left, v);
+    };
+
+    MxLinB<NJ> B0, B1;
+    uint32_t sb[NJ];
+    if (resident) {
+        loadb(B0, 0, 4 * wk);                                     // in flight while the rows are quantised
+        loads(sb, 0, wk);
+        stage(0, g.S);
+        __syncthreads();
+    }
+    constexpr int LPR = EPN / 8, RPI = 64 / LPR, NQ = 16 / RPI;   // lanes per staged row, rows per wave instruction, instructions per 16 rows
+    for (int it = 0; it < g.per_wg; ++it) {
+        const int n0 = ((blockIdx.y * g.per_wg + it) * WN + wn) * EPN;
+        if (resident && WK == 1 && n0 >= g.N) break;              // (no barrier below in that form)
+        const int nl = WK > 1 ? tid % LPR : lane % LPR, nc = n0 + nl * 8, left = g.N - nc;
+        // the residual rows are asked for before the products: their latency is the longest here
+        MxRaw8<T> rv[WK == 1 ? MI * 2 * NQ : 1];
+        if (WK == 1 && g.res) {
+#pragma unroll
+            for (int q = 0; q < MI * 2 * NQ; ++q) {
+                const int64_t m = m0 + wm * MI * 32 + q * RPI + lane / LPR;
+                rv[q].template load<FULL>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M);
             }
         }
-        if (!live) continue;
-
-        // 32 rows at a time through LDS (a wave's own slice: no barrier), then 8 columns a lane
-        const int n0 = tile * 64, nc = n0 + (lane & 7) * 8, left = g.N - nc;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+        for (int s0 = 0; s0 < g.S; s0 += resident ? g.S : g.chunk) {
+            const int s1 = resident || s0 + g.chunk > g.S ? g.S : s0 + g.chunk;
+            int s = s0 + 4 * wk;
+            if (!resident) {
+                __syncthreads();
+                loadb(B0, it, s);
+                loads(sb, it, s >> 2);
+                stage(s0, s1);
+                __syncthreads();
+            }
+            for (; s < s1; s += 4 * WK) {
+                uint32_t sa[MI], sn[NJ];
+#pragma unroll
+                for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(srow + i * 32 * g.spitch + ((s - s0) >> 2) * 8);
+                loadb(B1, it, s + 2);
+                loads(sn, it, (s >> 2) + WK);
+                MXL_STEP(B0, 0, 0) MXL_STEP(B0, 1, 1)
+                loadb(B0, it, s + 4 * WK);
+                s += 2;
+                MXL_STEP(B1, 0, 2) MXL_STEP(B1, 1, 3)
+                s -= 2;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) sb[j] = sn[j];
+            }
+        }
+        if (resident && it + 1 < g.per_wg) {
+            loadb(B0, it + 1, 4 * wk);
+            loads(sb, it + 1, wk);
+        }
         float bs[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bs[e] = (g.bias && e < left) ? g.bias[nc + e] : 0.f;
+        for (int e = 0; e < 8; ++e) bs[e] = 0.f;
+        if (g.bias) {
+            MxRaw8<float> b;
+            b.template load<FULL>(g.bias, nc, left, true);
+            b.get(bs);
+        }
+        if (WK == 1) {
+            // 16 rows at a time through the wave's own slice of LDS, then eight columns a lane
+            float* ep = reinterpret_cast<float*>(smem + g.ep_ofs) + wave * 16 * EPP;
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int h = 0; h < 2; ++h) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ep[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * MXL_EP + j * 32 + (lane & 31)] = acc[i][j][e];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int r = q * 8 + (lane >> 3);
-                const int64_t m = m0 + (wm * MI + i) * 32 + r;
-                float v[8];
-                const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + r * MXL_EP + (lane & 7) * 8);
-                const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(ep + r * MXL_EP + (lane & 7) * 8 + 4);
+                        for (int e = 0; e < 8; ++e) ep[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[i][j][8 * h + e];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { v[e] = lo[e] + bs[e]; v[4 + e] = hi[e] + bs[4 + e]; }
-                if (m < g.M && left > 0) {
-                    if (g.res) {
-                        float rv[8];
-                        mx_load8(reinterpret_cast<const T*>(g.res) + m * g.N + nc, left, rv);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += rv[e];
+                    for (int q = 0; q < NQ; ++q) {
+                        const int r = q * RPI + lane / LPR;
+                        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + r * EPP + nl * 8), hi = *reinterpret_cast<const f32x4_t*>(ep + r * EPP + nl * 8 + 4);
+                        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                        finish(v, rv[(i * 2 + h) * NQ + q], m0 + (wm * MI + i) * 32 + h * 16 + r, nc, left, bs);
                     }
-                    if (g.relu) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];        // (a NaN stays one)
-                    }
-                    mx_store8(reinterpret_cast<T*>(g.y) + m * g.N + nc, left, v);
                 }
+        } else {
+            float* ep = reinterpret_cast<float*>(smem + g.ep_ofs);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ep[(wk * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[0][j][e];
+            __syncthreads();
+            for (int r = tid / LPR; r < rows; r += 256 / LPR) {
+                if (g.res) rv[0].template load<FULL>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < WK; ++k) {
+                    const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8), hi = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8 + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
+                }
+                finish(v, rv[0], m0 + r, nc, left, bs);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
+#undef MXL_STEP
 }
 
-template <typename T, int BM, int WM>
+template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULL>
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
-    constexpr int WN = 4 / WM;
-    // LDS: at most 1024 steps' worth is never needed; hold as many channels as fit beside the output staging
-    const int ep = 4 * 32 * MXL_EP * 4;
+    constexpr int BM = 32 * MI * WM, EPP = 32 * NJ + 4;
+    const int ep = (WK > 1 ? 4 * 32 : 4 * 16) * EPP * 4;
+    // LDS holds all channels of the rows where they fit, else a chunk at a time
     int chunk = g.S;
-    auto bytes = [&](int c, int* pitch, int* spitch) {
-        *pitch = c * 32 + 16;                       // an odd number of 16-byte pieces: eight rows' reads hit different banks
-        *spitch = cdiv(c, 4) * 8 + 4;
-        return BM * (*pitch + *spitch);
+    auto bytes = [&](int c) {
+        g.pitch = c * 32 + 16;                      // an odd number of 16-byte pieces: eight rows' reads hit different banks
+        g.spitch = cdiv(c, 4) * 8 + 4;
+        return BM * (g.pitch + g.spitch);
     };
-    while (bytes(chunk, &g.pitch, &g.spitch) + ep > 150 * 1024) chunk = chunk > 64 ? 64 : chunk / 2 / 4 * 4;
+    while (bytes(chunk) + ep > 150 * 1024) chunk = chunk > 128 ? 128 : chunk / 2 / 4 * 4;
     g.chunk = chunk;
     g.sc_ofs = BM * g.pitch;
     g.ep_ofs = (BM * (g.pitch + g.spitch) + 15) / 16 * 16;
     const int smem = g.ep_ofs + ep;
-    g.cdiv_full = mx_div((uint32_t)chunk * 8);
-    const int last = g.S % chunk ? g.S % chunk : chunk;
-    g.cdiv_last = mx_div((uint32_t)last * 8);
-    g.ntiles = cdiv(g.N, 64);
+    g.div_full = mx_div((uint32_t)chunk * 8);
+    g.div_last = mx_div((uint32_t)(g.S % chunk ? g.S % chunk : chunk) * 8);
+    g.t32 = cdiv(g.N, 32);
     const int64_t mt = (g.M + BM - 1) / BM;
     if (mt >= ((int64_t)1 << 31)) { cn_set_error("cn_mx_linear_fwd: too many rows"); return CN_EINVAL; }
-    const int passes = cdiv(g.ntiles, WN);
+    const int passes = cdiv(g.t32, NJ * WN);
     // one workgroup walks all columns of its rows unless that leaves compute units idle
-    int split = (int)(mt >= 512 ? 1 : (512 + mt - 1) / mt);
-    split = chunk < g.S ? passes : (split < passes ? split : passes);
+    int64_t split = mt >= 1024 ? 1 : (1024 + mt - 1) / mt;
+    if (chunk < g.S || split > passes) split = passes;
     g.per_wg = cdiv(passes, split);
     split = cdiv(passes, g.per_wg);
     static bool attr[64] = {};
     int dev = 0;
-    (void)hipGetDevice(&dev);
-    dev &= 63;
-    if (!attr[dev]) {
-        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, BM, WM>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        attr[dev] = true;
+    CN_HIP(hipGetDevice(&dev));
+    if (dev >= 64 || !attr[dev]) {
+        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if (dev < 64) attr[dev] = true;
     }
-    mx_linear_kernel<T, BM, WM><<<dim3((unsigned)mt, split), 256, smem, st>>>(g);
+    const dim3 grid((unsigned)mt, (unsigned)split);
+    if (chunk >= g.S) mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, true><<<grid, 256, smem, st>>>(g);
+    else mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, false><<<grid, 256, smem, st>>>(g);
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
+}
+template <typename T, bool FULL>
+static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
+    // few rows: less than one 64 x 256 workgroup for each compute unit
+    if ((g.M + 63) / 64 * cdiv(g.N, 256) < 256) return mxl_launch<T, 1, 1, 1, 1, 4, FULL>(g, st);
+    if (g.N <= 64) return mxl_launch<T, 1, 2, 4, 1, 1, FULL>(g, st);
+    if (g.N <= 128) return mxl_launch<T, 1, 2, 2, 2, 1, FULL>(g, st);
+    return mxl_launch<T, 1, 2, 1, 4, 1, FULL>(g, st);
 }
 
 extern "C" int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const void* residual, void* y, int64_t M, int K, int N,
@@ -277,11 +356,6 @@ extern "C" int cn_mx_linear_fwd(const void* x, const void* packed, const float* 
     g.S4 = cdiv(g.S, 4);
     g.relu = relu;
     hipStream_t st = (hipStream_t)stream;
-#define MXL_GO(BM, WM) return dtype == CN_BF16 ? mxl_launch<bf16_t, BM, WM>(g, st) : mxl_launch<float, BM, WM>(g, st)
-    if (M <= 64) { MXL_GO(32, 1); }
-    if (N <= 64) { MXL_GO(128, 4); }
-    if (N <= 128) { MXL_GO(128, 2); }
-    if (K <= 512) { MXL_GO(128, 1); }
-    MXL_GO(64, 1);
-#undef MXL_GO
+    if (dtype == CN_BF16) return (K | N) % 8 == 0 ? mxl_choose<bf16_t, true>(g, st) : mxl_choose<bf16_t, false>(g, st);
+    return (K | N) % 8 == 0 ? mxl_choose<float, true>(g, st) : mxl_choose<float, false>(g, st);
 }

@@ -35,62 +35,30 @@ struct MxWgGeom {
     int ktiles, accumulate;
 };
 
-// Eight raw dy elements; FULL: N is a multiple of 8, a chunk is inside the row or outside (branch-free: a readable address, masked)
-template <typename T> struct MxRaw8;
-template <> struct MxRaw8<bf16_t> {
-    uint4 a;
-    template <bool FULL> __device__ inline void load(const bf16_t* base, int64_t at, int left, bool ok) {
-        if (FULL) {
-            ok = ok && left > 0;
-            const u32x4_t v = *reinterpret_cast<const u32x4_a2*>(base + (ok ? at : 0));
-            const uint32_t m = ok ? 0xffffffffu : 0u;
-            a = make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
-        } else {
-            float f[8];
-            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
-            a = make_uint4(pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7]));
-        }
-    }
-    __device__ inline void get(float (&f)[8]) const { Vec16<bf16_t>::unpack(a, f); }
-    __device__ inline void put(bf16_t* lds, int) const { st16(lds, a); }
-};
-template <> struct MxRaw8<float> {
+// a loaded dy chunk into its LDS plane(s)
+__device__ static inline void mx_put_dy(const MxRaw8<bf16_t>& r, bf16_t* lds, int) { *reinterpret_cast<u32x4_t*>(lds) = r.a; }
+// 32 bits: three planes, `plane` elements apart: truncation to 8 significant bits twice, the rest is exact; an infinity or a NaN is all in
+// the first
+__device__ static inline void mx_put_dy(const MxRaw8<float>& r, bf16_t* lds, int plane) {
     float f[8];
-    template <bool FULL> __device__ inline void load(const float* base, int64_t at, int left, bool ok) {
-        if (FULL) {
-            ok = ok && left > 0;
-            const float* p = base + (ok ? at : 0);
-            const u32x4_t v = *reinterpret_cast<const u32x4_a4*>(p), w = *reinterpret_cast<const u32x4_a4*>(p + 4);
-            const uint32_t m = ok ? 0xffffffffu : 0u;
+    r.get(f);
+    uint32_t h[8], m[8], l[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(v[i] & m); f[4 + i] = __uint_as_float(w[i] & m); }
-        } else {
-            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
-        }
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = __float_as_uint(f[i]);
+        const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+        h[i] = fin ? u & 0xffff0000u : ((u & 0x7fffffu) ? 0x7fc00000u : u);
+        const float d = fin ? f[i] - __uint_as_float(h[i]) : 0.f;
+        m[i] = __float_as_uint(d) & 0xffff0000u;
+        l[i] = __float_as_uint(d - __uint_as_float(m[i]));
     }
-    __device__ inline void get(float (&o)[8]) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = f[i];
-    }
-    // three planes, `plane` elements apart: truncation to 8 significant bits twice, the rest is exact; an infinity or NaN is all in the first
-    __device__ inline void put(bf16_t* lds, int plane) const {
-        uint32_t h[8], m[8], l[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t u = __float_as_uint(f[i]);
-            const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-            h[i] = fin ? u & 0xffff0000u : ((u & 0x7fffffu) ? 0x7fc00000u : u);
-            const float r = fin ? f[i] - __uint_as_float(h[i]) : 0.f;
-            m[i] = __float_as_uint(r) & 0xffff0000u;
-            l[i] = __float_as_uint(r - __uint_as_float(m[i]));
-        }
-#define MX_PK(x) make_uint4((x[0] >> 16) | (x[1] & 0xffff0000u), (x[2] >> 16) | (x[3] & 0xffff0000u), (x[4] >> 16) | (x[5] & 0xffff0000u), (x[6] >> 16) | (x[7] & 0xffff0000u))
-        st16(lds, MX_PK(h));
-        st16(lds + plane, MX_PK(m));
-        st16(lds + 2 * plane, MX_PK(l));
-#undef MX_PK
-    }
-};
+    auto pk = [](const uint32_t (&x)[8]) {
+        return u32x4_t{(x[0] >> 16) | (x[1] & 0xffff0000u), (x[2] >> 16) | (x[3] & 0xffff0000u), (x[4] >> 16) | (x[5] & 0xffff0000u), (x[6] >> 16) | (x[7] & 0xffff0000u)};
+    };
+    *reinterpret_cast<u32x4_t*>(lds) = pk(h);
+    *reinterpret_cast<u32x4_t*>(lds + plane) = pk(m);
+    *reinterpret_cast<u32x4_t*>(lds + 2 * plane) = pk(l);
+}
 
 template <typename T, int TN, int TK, bool FULL>
 __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
@@ -140,7 +108,7 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     auto lstore = [&]() {
 #pragma unroll
         for (int v = 0; v < YV; ++v) {
-            ry[v].put(ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
+            mx_put_dy(ry[v], ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
             if (bias) {
                 float f[8];
                 ry[v].get(f);

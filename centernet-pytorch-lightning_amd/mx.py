@@ -18,40 +18,59 @@ value = round-to-nearest-even(x / scale) * scale, in the type asked for (next to
 import torch
 
 from . import _hip
-from ._hip import call, dtype_code
+from ._hip import launch
 
 BLOCK = 32
 FORMATS = {"e2m1": 0, "e4m3": 1}          # CN_MX_E2M1, CN_MX_E4M3
 MAX_CHANNELS = 65536
+_DTYPES = {torch.float32: _hip.CN_F32, torch.bfloat16: _hip.CN_BF16}
 
 
 class MXTensor:
     """A quantised tensor: `codes` uint8 [rows, Cp * bits / 8] (Cp = channels rounded up to 32), `scales` uint8 [rows, Cp / 32], the
-    `shape` and `dtype` it was made from, and optionally `signs` uint8 [rows, Cp / 8] (see `checkpoint`)."""
-    __slots__ = ("codes", "scales", "signs", "shape", "dtype", "fmt")
+    `shape` and `dtype` it was made from, and optionally `signs` uint8 [rows, Cp / 8] (see `checkpoint`) — three views of one buffer."""
+    __slots__ = ("buffer", "shape", "dtype", "fmt", "rows", "blocks", "has_signs", "_n")
 
-    def __init__(self, codes, scales, shape, dtype, fmt, signs=None):
-        self.codes, self.scales, self.signs = codes, scales, signs
-        self.shape, self.dtype, self.fmt = torch.Size(shape), dtype, fmt
+    def __init__(self, shape, dtype, fmt, device, signs=False):
+        self.shape, self.dtype, self.fmt, self.has_signs = shape, dtype, fmt, signs
+        self.blocks = (shape[-1] + BLOCK - 1) // BLOCK
+        self.rows = shape[:-1].numel()
+        self._n = self.rows * self.blocks                  # blocks in all
+        self.buffer = torch.empty(self._n * ((33 if fmt == "e4m3" else 17) + (4 if signs else 0)), dtype=torch.uint8, device=device)
+
+    def _pointers(self):
+        """codes, scales, signs (None without)"""
+        p = self.buffer.data_ptr()
+        s = p + self._n * (32 if self.fmt == "e4m3" else 16)
+        return p, s, s + self._n if self.has_signs else None
+
+    def _part(self, first, width):
+        return self.buffer[self._n * first:self._n * (first + width)].view(self.rows, self.blocks * width)
+
+    @property
+    def codes(self):
+        return self._part(0, 32 if self.fmt == "e4m3" else 16)
+
+    @property
+    def scales(self):
+        return self._part(32 if self.fmt == "e4m3" else 16, 1)
+
+    @property
+    def signs(self):
+        return self._part(33 if self.fmt == "e4m3" else 17, 4) if self.has_signs else None
 
     @property
     def device(self):
-        return self.codes.device
-
-    @property
-    def rows(self):
-        return self.codes.shape[0]
+        return self.buffer.device
 
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel() + (self.signs.numel() if self.signs is not None else 0)
+        return self.buffer.numel()
 
     def record_stream(self, stream):
-        for t in (self.codes, self.scales, self.signs):
-            if t is not None:
-                t.record_stream(stream)
+        self.buffer.record_stream(stream)
 
     def __repr__(self):
-        return f"MXTensor({self.fmt}, {tuple(self.shape)}, {self.dtype}{', signs' if self.signs is not None else ''})"
+        return f"MXTensor({self.fmt}, {tuple(self.shape)}, {self.dtype}{', signs' if self.has_signs else ''})"
 
 
 class MXWeight:
@@ -66,24 +85,30 @@ class MXWeight:
 
 
 def _tensor(t, what):
+    """-> (t contiguous, dtype code), or an error"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
-    dtype_code(t.dtype)                                    # bf16 / fp32, else TypeError
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype} (bfloat16 or float32)")
     if t.dim() < 1 or not 1 <= t.shape[-1] <= MAX_CHANNELS:
         raise ValueError(f"{what}: expected [..., 1 .. {MAX_CHANNELS} channels], got {tuple(t.shape)}")
     if not t.is_cuda:
         raise RuntimeError(f"{what}: tensor is not on the GPU (no CPU path exists)")
-    return t.detach().contiguous()
+    return (t if t.is_contiguous() else t.contiguous()), code
 
 
-def _like(t, ref, what, shape=None, dtype=None):
-    """`t` as a contiguous tensor with ref's device and the wanted shape / dtype, or an error"""
-    shape, dtype = ref.shape if shape is None else shape, dtype or ref.dtype
+def _like(t, device, shape, dtype, what):
+    """t contiguous if it is a tensor of that device, shape and type, else an error"""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what}: expected a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != ref.device:
-        raise ValueError(f"{what}: expected {tuple(shape)} {dtype} on {ref.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.detach().contiguous()
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: expected {tuple(shape)} {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _fmt(fmt):
@@ -92,39 +117,26 @@ def _fmt(fmt):
     return FORMATS[fmt]
 
 
-def _rows(t):
-    return t.numel() // t.shape[-1]
-
-
-def _empty(n, dtype, device):
-    return torch.empty(n, dtype=dtype, device=device)
-
-
 def quantize(x, fmt="e4m3"):
     """x [..., C] -> MXTensor.  One pass: x is read once, codes and scales are written."""
-    return _quantize(x, fmt, None)
+    return _quantize(x, fmt, None, "mx.quantize")
 
 
 def checkpoint(x, sign_of=None):
     """x [..., C] -> e4m3 MXTensor for the backward pass: 8.25 bits a value instead of 16 or 32.  sign_of: the tensor (x's shape and
     dtype) whose positive entries a ReLU let through; one bit of each is kept with the codes."""
-    return _quantize(x, "e4m3", sign_of)
+    return _quantize(x, "e4m3", sign_of, "mx.checkpoint")
 
 
-def _quantize(x, fmt, sign_of):
+def _quantize(x, fmt, sign_of, what):
     code = _fmt(fmt)
-    x = _tensor(x, "mx.quantize")
+    x, dt = _tensor(x, what)
     if sign_of is not None:
-        sign_of = _like(sign_of, x, "mx.checkpoint: sign_of")
-    rows, C = _rows(x), x.shape[-1]
-    blocks = (C + BLOCK - 1) // BLOCK
-    with torch.cuda.device(x.device):
-        codes = _empty((rows, blocks * (32 if code else 16)), torch.uint8, x.device)
-        scales = _empty((rows, blocks), torch.uint8, x.device)
-        signs = _empty((rows, blocks * 4), torch.uint8, x.device) if sign_of is not None else None
-        if rows:
-            call("cn_mx_quantize", x, codes, scales, sign_of, signs, rows, C, code, dtype_code(x.dtype))
-    return MXTensor(codes, scales, x.shape, x.dtype, fmt, signs)
+        sign_of = _like(sign_of, x.device, x.shape, x.dtype, "mx.checkpoint: sign_of")
+    q = MXTensor(x.shape, x.dtype, fmt, x.device, sign_of is not None)
+    codes, scales, signs = q._pointers()
+    launch("cn_mx_quantize", x.get_device(), x.data_ptr(), codes, scales, _ptr(sign_of), signs, q.rows, x.shape[-1], code, dt)
+    return q
 
 
 def dequantize(q, dtype=None):
@@ -132,11 +144,11 @@ def dequantize(q, dtype=None):
     if not isinstance(q, MXTensor):
         raise TypeError(f"mx.dequantize: expected an MXTensor, got {type(q).__name__}")
     dtype = dtype or q.dtype
-    code = dtype_code(dtype)
-    with torch.cuda.device(q.device):
-        out = _empty(q.shape, dtype, q.device)
-        if out.numel():
-            call("cn_mx_dequantize", q.codes, q.scales, out, q.rows, q.shape[-1], _fmt(q.fmt), code)
+    if dtype not in _DTYPES:
+        raise TypeError(f"mx.dequantize: unsupported dtype {dtype} (bfloat16 or float32)")
+    out = torch.empty(q.shape, dtype=dtype, device=q.buffer.device)
+    codes, scales, _ = q._pointers()
+    launch("cn_mx_dequantize", out.get_device(), codes, scales, out.data_ptr(), q.rows, q.shape[-1], FORMATS[q.fmt], _DTYPES[dtype])
     return out
 
 
@@ -148,13 +160,12 @@ def pack_weight(weight):
         weight = weight.reshape(weight.shape[0], weight.shape[1])
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("mx.pack_weight: expected [out_features, in_features]")
-    w = _tensor(weight, "mx.pack_weight")
+    w, dt = _tensor(weight, "mx.pack_weight")
     N, K = w.shape
     if not 1 <= N <= MAX_CHANNELS:
         raise ValueError(f"mx.pack_weight: out_features {N} not in 1 .. {MAX_CHANNELS}")
-    with torch.cuda.device(w.device):
-        packed = _empty(int(_hip.query("cn_mx_weight_bytes", N, K)), torch.uint8, w.device)
-        call("cn_mx_pack_weight", w, packed, N, K, dtype_code(w.dtype))
+    packed = torch.empty(_hip.query("cn_mx_weight_bytes", N, K), dtype=torch.uint8, device=w.device)
+    launch("cn_mx_pack_weight", w.get_device(), w.data_ptr(), packed.data_ptr(), N, K, dt)
     return MXWeight(packed, N, K)
 
 
@@ -165,21 +176,21 @@ def linear(x, weight, bias=None, residual=None, relu=False):
         raise TypeError("mx.linear: weight must come from mx.pack_weight")
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, bias, residual)):
         raise RuntimeError("mx.linear has no backward pass: call it under torch.no_grad()")
-    x = _tensor(x, "mx.linear")
-    N, K = weight.out_features, weight.in_features
+    x, dt = _tensor(x, "mx.linear")
+    N, K, dev = weight.out_features, weight.in_features, x.device
     if x.shape[-1] != K:
         raise ValueError(f"mx.linear: x has {x.shape[-1]} channels, weight expects {K}")
-    if weight.packed.device != x.device:
-        raise ValueError(f"mx.linear: weight on {weight.packed.device}, x on {x.device}")
-    shape = (*x.shape[:-1], N)
+    if weight.packed.device != dev:
+        raise ValueError(f"mx.linear: weight on {weight.packed.device}, x on {dev}")
+    lead = x.shape[:-1]
+    shape = (*lead, N)
     if bias is not None:
-        bias = _like(bias, x, "mx.linear: bias", (N,), torch.float32)
+        bias = _like(bias, dev, (N,), torch.float32, "mx.linear: bias")
     if residual is not None:
-        residual = _like(residual, x, "mx.linear: residual", shape)
-    with torch.cuda.device(x.device):
-        y = _empty(shape, x.dtype, x.device)
-        if y.numel():
-            call("cn_mx_linear_fwd", x, weight.packed, bias, residual, y, _rows(x), K, N, int(bool(relu)), dtype_code(x.dtype))
+        residual = _like(residual, dev, shape, x.dtype, "mx.linear: residual")
+    y = torch.empty(shape, dtype=x.dtype, device=dev)
+    launch("cn_mx_linear_fwd", x.get_device(), x.data_ptr(), weight.packed.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), lead.numel(),
+           K, N, 1 if relu else 0, dt)
     return y
 
 
@@ -193,30 +204,29 @@ def _checkpoint_of(ck, dy, what):
 def linear_wgrad(dy, ck, bias=False, into=None, bias_into=None):
     """Gradients of a linear layer / 1x1 convolution whose input was kept as `ck`: -> (dw fp32 [N, K], db fp32 [N] | None) for
     dy [..., N].  into / bias_into: contiguous fp32 tensors (of N * K / N values) the gradients are added to instead."""
-    dy = _tensor(dy, "mx.linear_wgrad")
+    dy, dt = _tensor(dy, "mx.linear_wgrad")
     _checkpoint_of(ck, dy, "mx.linear_wgrad")
     if dy.shape[:-1] != ck.shape[:-1]:
         raise ValueError(f"mx.linear_wgrad: gradient {tuple(dy.shape)} and checkpoint {tuple(ck.shape)} have different rows")
-    rows, N, K = ck.rows, dy.shape[-1], ck.shape[-1]
+    rows, N, K, dev = ck.rows, dy.shape[-1], ck.shape[-1], dy.device
     for t, n, what in ((into, N * K, "into"), (bias_into, N, "bias_into")):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != dy.device or not t.is_contiguous()):
-            raise ValueError(f"mx.linear_wgrad: {what} must be contiguous fp32 with {n} values on {dy.device}")
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != dev or not t.is_contiguous()):
+            raise ValueError(f"mx.linear_wgrad: {what} must be contiguous fp32 with {n} values on {dev}")
     if bias_into is not None and into is None or into is not None and bias and bias_into is None:
         raise ValueError("mx.linear_wgrad: into and bias_into come together when a bias gradient is wanted")
-    want_b = bool(bias) or bias_into is not None
-    dt = dtype_code(dy.dtype)
-    with torch.cuda.device(dy.device):
-        dw = into if into is not None else _empty((N, K), torch.float32, dy.device)
-        db = bias_into if bias_into is not None else (_empty((N,), torch.float32, dy.device) if want_b else None)
-        if rows == 0:
-            if into is None:
-                dw.zero_()
-                if db is not None:
-                    db.zero_()
-        else:
-            n = int(_hip.query("cn_mx_linear_wgrad_bytes", rows, K, N, dt))
-            ws = _empty(n, torch.uint8, dy.device)
-            call("cn_mx_linear_wgrad", dy, ck.codes, ck.scales, dw, db, int(into is not None), rows, K, N, dt, ws, n)
+    dw = into if into is not None else torch.empty((N, K), dtype=torch.float32, device=dev)
+    db = bias_into if bias_into is not None else (torch.empty((N,), dtype=torch.float32, device=dev) if bias else None)
+    if rows == 0:
+        if into is None:
+            dw.zero_()
+            if db is not None:
+                db.zero_()
+        return dw, db
+    n = _hip.query("cn_mx_linear_wgrad_bytes", rows, K, N, dt)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    codes, scales, _ = ck._pointers()
+    launch("cn_mx_linear_wgrad", dy.get_device(), dy.data_ptr(), codes, scales, dw.data_ptr(), _ptr(db), 0 if into is None else 1, rows, K, N,
+           dt, ws.data_ptr(), n)
     return dw, db
 
 
@@ -224,29 +234,32 @@ def batch_norm_act_bwd(dy, ck, gamma, mean, invstd, residual=False, racc=None, i
     """Backward of y = [relu](gamma * (x - mean) * invstd + beta [+ residual]) with batch statistics over the rows, from ck =
     mx.checkpoint(x, sign_of=y) (sign_of=None: no ReLU): -> (dx, dgamma, dbeta, dres).  residual: also return the residual input's
     gradient (racc: a tensor to add to it), else dres is None.  into: (gamma.grad, beta.grad) to add to instead of new tensors."""
-    dy = _tensor(dy, "mx.batch_norm_act_bwd")
+    dy, dt = _tensor(dy, "mx.batch_norm_act_bwd")
     _checkpoint_of(ck, dy, "mx.batch_norm_act_bwd")
     if dy.shape != ck.shape or dy.dtype != ck.dtype:
         raise ValueError(f"mx.batch_norm_act_bwd: gradient {tuple(dy.shape)} {dy.dtype}, checkpoint of {tuple(ck.shape)} {ck.dtype}")
-    rows, C = ck.rows, ck.shape[-1]
+    rows, C, dev, one = ck.rows, ck.shape[-1], dy.device, (ck.shape[-1],)
     if rows == 0:
         raise ValueError("mx.batch_norm_act_bwd: no rows (batch statistics are undefined)")
     if racc is not None and not residual:
         raise ValueError("mx.batch_norm_act_bwd: racc without residual")
-    gamma, mean, invstd = (_like(t, dy, f"mx.batch_norm_act_bwd: {n}", (C,), torch.float32)
-                           for t, n in ((gamma, "gamma"), (mean, "mean"), (invstd, "invstd")))
+    gamma = _like(gamma, dev, one, torch.float32, "mx.batch_norm_act_bwd: gamma")
+    mean = _like(mean, dev, one, torch.float32, "mx.batch_norm_act_bwd: mean")
+    invstd = _like(invstd, dev, one, torch.float32, "mx.batch_norm_act_bwd: invstd")
     if racc is not None:
-        racc = _like(racc, dy, "mx.batch_norm_act_bwd: racc")
+        racc = _like(racc, dev, dy.shape, dy.dtype, "mx.batch_norm_act_bwd: racc")
     if into is not None:
+        dgamma, dbeta = into
         for t in into:
-            if _like(t, dy, "mx.batch_norm_act_bwd: into", (C,), torch.float32).data_ptr() != t.data_ptr():
+            if _like(t, dev, one, torch.float32, "mx.batch_norm_act_bwd: into") is not t:
                 raise ValueError("mx.batch_norm_act_bwd: into must be contiguous")
-    with torch.cuda.device(dy.device):
-        dx = torch.empty_like(dy)
-        dres = torch.empty_like(dy) if residual else None
-        dgamma, dbeta = into if into is not None else (_empty((C,), torch.float32, dy.device) for _ in range(2))
-        n = int(_hip.query("cn_mx_bn_bwd_bytes", rows, C))
-        ws = _empty(n, torch.uint8, dy.device)
-        call("cn_mx_bn_bwd", dy, ck.codes, ck.scales, ck.signs, gamma, mean, invstd, dx, dres, racc, dgamma, dbeta,
-             int(into is not None), rows, C, dtype_code(dy.dtype), ws, n)
+    else:
+        dgamma, dbeta = torch.empty(one, dtype=torch.float32, device=dev), torch.empty(one, dtype=torch.float32, device=dev)
+    dx = torch.empty_like(dy)
+    dres = torch.empty_like(dy) if residual else None
+    n = _hip.query("cn_mx_bn_bwd_bytes", rows, C)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    codes, scales, signs = ck._pointers()
+    launch("cn_mx_bn_bwd", dy.get_device(), dy.data_ptr(), codes, scales, signs, gamma.data_ptr(), mean.data_ptr(), invstd.data_ptr(),
+           dx.data_ptr(), _ptr(dres), _ptr(racc), dgamma.data_ptr(), dbeta.data_ptr(), 0 if into is None else 1, rows, C, dt, ws.data_ptr(), n)
     return dx, dgamma, dbeta, dres
