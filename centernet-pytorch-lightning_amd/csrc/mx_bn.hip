@@ -22,22 +22,32 @@ struct MxBnGeom {
     int64_t per;               // rows per workgroup
 };
 
-// one row's d and x8 of a thread's chunk
-template <typename T, bool SIGNS>
-__device__ static inline void mxbn_load(const MxBnGeom& g, int64_t r, int c, int left, float (&d)[8], float (&v)[8]) {
-    const int64_t i = r * g.cpr + c;
-    const uint2 q = reinterpret_cast<const uint2*>(g.codes)[i];
-    const uint32_t b = g.scales[r * g.blocks + (c >> 2)];
-    mx_load8(reinterpret_cast<const T*>(g.dy) + r * g.C + c * 8, left, d);
-    if (SIGNS) {
-        const uint32_t m = g.signs[i];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = (m >> j) & 1 ? d[j] : 0.f;
-    }
-    mx_values_e4m3(q.x, q.y, mx_scale_value(b), v);
-}
+#define MXBN_U 4               // rows a thread has in flight
 
-template <typename T, bool SIGNS>
+// a row's dy, codes, scale and sign bits for a thread's chunk, as they lie in memory
+template <typename T> struct MxBnRow {
+    MxRaw8<T> dy;
+    uint2 q;
+    uint32_t b, m;
+    template <bool SIGNS, bool FULL> __device__ inline void load(const MxBnGeom& g, int64_t r, int c, int left, bool ok) {
+        r = ok ? r : 0;                                           // (row 0 is readable; its values are not used then)
+        const int64_t i = r * g.cpr + c;
+        q = reinterpret_cast<const uint2*>(g.codes)[i];
+        b = g.scales[r * g.blocks + (c >> 2)];
+        m = SIGNS ? g.signs[i] : 0u;
+        dy.template load<FULL>(reinterpret_cast<const T*>(g.dy), r * g.C + c * 8, left, true);
+    }
+    template <bool SIGNS> __device__ inline void get(float (&d)[8], float (&v)[8]) const {
+        dy.get(d);
+        if (SIGNS) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d[j] = (m >> j) & 1 ? d[j] : 0.f;
+        }
+        mx_values_e4m3(q.x, q.y, mx_scale_value(b), v);
+    }
+};
+
+template <typename T, bool SIGNS, bool FULL>
 __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const float* __restrict__ mean, float* __restrict__ part) {
     __shared__ float red[4 * 32 * 16];
     const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
@@ -47,12 +57,19 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
 #pragma unroll
     for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; mu[j] = j < left ? mean[c * 8 + j] : 0.f; }
     if (left > 0) {
-#pragma unroll 4
-        for (int64_t r = r0 + rl; r < r1; r += nrl) {
-            float d[8], v[8];
-            mxbn_load<T, SIGNS>(g, r, c, left, d, v);
+        for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
+            MxBnRow<T> row[MXBN_U];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
+            for (int u = 0; u < MXBN_U; ++u) row[u].template load<SIGNS, FULL>(g, r + u * nrl, c, left, r + u * nrl < r1);
+#pragma unroll
+            for (int u = 0; u < MXBN_U; ++u) {
+                if (r + u * nrl < r1) {
+                    float d[8], v[8];
+                    row[u].template get<SIGNS>(d, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
+                }
+            }
         }
     }
     // lanes of one chunk within the wave, then the four waves
@@ -73,28 +90,42 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
     }
 }
 
-// 32 channels x 8 partial rows per workgroup: totals, parameter gradients, and the coefficients a, b, c of dx
+// 16 channels x 64 partial rows per workgroup: totals, parameter gradients, and the coefficients a, b, c of dx
 __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, float inv_rows,
                                                            const float* __restrict__ gamma, const float* __restrict__ invstd,
                                                            float* __restrict__ coef, float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                            int accumulate) {
-    __shared__ float red[2][8][32];
-    const int cl = threadIdx.x & 31, gl = threadIdx.x >> 5, ch = blockIdx.x * 32 + cl;
-    float s0 = 0.f, s1 = 0.f;
-    if (ch < C) {
-#pragma unroll 4
-        for (int g = gl; g < groups; g += 8) {
-            s0 += part[(int64_t)g * 2 * C + ch];
-            s1 += part[((int64_t)g * 2 + 1) * C + ch];
-        }
-    }
-    red[0][gl][cl] = s0;
-    red[1][gl][cl] = s1;
-    __syncthreads();
-    if (gl == 0 && ch < C) {
-        s0 = s1 = 0.f;
+    __shared__ float red[64][2][17];
+    const int cl = (threadIdx.x & 3) * 4, gl = threadIdx.x >> 2, c0 = blockIdx.x * 16;
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    int at[4];                                                     // (channels behind the last read the last one's sums; they are dropped)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { s0 += red[0][k][cl]; s1 += red[1][k][cl]; }
+    for (int j = 0; j < 4; ++j) at[j] = c0 + cl + j < C ? c0 + cl + j : C - 1;
+#pragma unroll 4
+    for (int g = gl; g < groups; g += 64) {
+        const float* p = part + (int64_t)g * 2 * C;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { s[0][j] += p[at[j]]; s[1][j] += p[C + at[j]]; }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[gl][k][cl + j] = s[k][j];
+    __syncthreads();
+    // 32 totals, eight threads each
+    const int o = threadIdx.x >> 3, q = threadIdx.x & 7, k = o >> 4, cc = o & 15;
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += red[q * 8 + i][k][cc];
+    t += __shfl_xor(t, 1, 64);
+    t += __shfl_xor(t, 2, 64);
+    t += __shfl_xor(t, 4, 64);
+    __syncthreads();
+    if (q == 0) red[0][k][cc] = t;
+    __syncthreads();
+    const int ch = c0 + threadIdx.x;
+    if (threadIdx.x < 16 && ch < C) {
+        const float s0 = red[0][0][threadIdx.x], s1 = red[0][1][threadIdx.x];
         const float is = invstd[ch], dg = s1 * is, a = gamma[ch] * is;
         coef[ch] = a;
         coef[C + ch] = a * is * dg * inv_rows;
@@ -104,7 +135,7 @@ __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restri
     }
 }
 
-template <typename T, bool SIGNS>
+template <typename T, bool SIGNS, bool FULL>
 __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, const float* __restrict__ mean, const float* __restrict__ coef,
                                                           T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc) {
     const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
@@ -112,30 +143,39 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
     if (left <= 0) return;
     const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
     float ka[8], kb[8], kc[8], mu[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int ch = c * 8 + j;
-        const bool ok = j < left;
-        ka[j] = ok ? coef[ch] : 0.f;
-        kb[j] = ok ? coef[g.C + ch] : 0.f;
-        kc[j] = ok ? coef[2 * g.C + ch] : 0.f;
-        mu[j] = ok ? mean[ch] : 0.f;
+    {
+        MxRaw8<float> k;
+        k.template load<FULL>(coef, c * 8, left, true);
+        k.get(ka);
+        k.template load<FULL>(coef, g.C + c * 8, left, true);
+        k.get(kb);
+        k.template load<FULL>(coef, 2 * g.C + c * 8, left, true);
+        k.get(kc);
+        k.template load<FULL>(mean, c * 8, left, true);
+        k.get(mu);
     }
-#pragma unroll 4
-    for (int64_t r = r0 + rl; r < r1; r += nrl) {
-        float d[8], v[8], o[8];
-        mxbn_load<T, SIGNS>(g, r, c, left, d, v);
-        const int64_t at = r * g.C + c * 8;
+    for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
+        MxBnRow<T> row[MXBN_U];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(ka[j], d[j], -fmaf(kb[j], v[j] - mu[j], kc[j]));
-        mx_store8(dx + at, left, o);
-        if (dres) {
-            if (racc) {
-                mx_load8(racc + at, left, o);
+        for (int u = 0; u < MXBN_U; ++u) row[u].template load<SIGNS, FULL>(g, r + u * nrl, c, left, r + u * nrl < r1);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) d[j] += o[j];
+        for (int u = 0; u < MXBN_U; ++u) {
+            if (r + u * nrl < r1) {
+                float d[8], v[8], o[8];
+                row[u].template get<SIGNS>(d, v);
+                const int64_t at = (r + u * nrl) * g.C + c * 8;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = fmaf(ka[j], d[j], -fmaf(kb[j], v[j] - mu[j], kc[j]));
+                mx_store8f<FULL>(dx + at, left, o);
+                if (dres) {
+                    if (racc) {
+                        mx_load8(racc + at, left, o);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] += o[j];
+                    }
+                    mx_store8f<FULL>(dres + at, left, d);
+                }
             }
-            mx_store8(dres + at, left, d);
         }
     }
 }
@@ -146,10 +186,10 @@ static int mxbn_lg(int C) {
     while (lg < 5 && (1 << lg) < chunks) ++lg;
     return lg;
 }
-// row groups of the sums pass: ~1024 workgroups in all, at least four rows for a thread
+// row groups of the sums pass: ~1024 workgroups in all, at least two rows for a thread
 static int mxbn_groups(int64_t rows, int C) {
     const int lg = mxbn_lg(C), tiles = cdiv(cdiv(C, 8), 1 << lg);
-    const int64_t most = (rows + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
+    const int64_t most = (rows + 2 * (256 >> lg) - 1) / (2 * (256 >> lg));
     int64_t g = 1024 / tiles;
     g = g < most ? g : most;
     return (int)(g < 1 ? 1 : (g > MXBN_MAX_GROUPS ? MXBN_MAX_GROUPS : g));
@@ -181,20 +221,24 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     const int nrl = 256 >> g.lg;
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
     g.per = (rows + groups - 1) / groups;
-    CN_DISPATCH_DTYPE(dtype, T, {
-        if (signs) mx_bn_sums_kernel<T, true><<<dim3(groups, tiles), 256, 0, st>>>(g, mean, part);
-        else mx_bn_sums_kernel<T, false><<<dim3(groups, tiles), 256, 0, st>>>(g, mean, part);
-    });
+    const bool full = C % 8 == 0;
+#define MXBN_GO(KERNEL, GRID, ...)                                                                                                     \
+    CN_DISPATCH_DTYPE(dtype, T, {                                                                                                      \
+        if (signs) { if (full) KERNEL<T, true, true><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, true, false><<<GRID, 256, 0, st>>>(__VA_ARGS__); }      \
+        else { if (full) KERNEL<T, false, true><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, false, false><<<GRID, 256, 0, st>>>(__VA_ARGS__); }          \
+    })
+    MXBN_GO(mx_bn_sums_kernel, dim3(groups, tiles), g, mean, part);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
-    mx_bn_finish_kernel<<<cdiv(C, 32), 256, 0, st>>>(part, groups, C, 1.f / (float)rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
+    mx_bn_finish_kernel<<<cdiv(C, 16), 256, 0, st>>>(part, groups, C, 1.f / (float)rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
-    g.per = 8 * nrl;
-    while ((rows + g.per - 1) / g.per > (int64_t)1 << 20) g.per *= 2;
+    // eight rows a thread (its coefficients are loaded once), fewer where that would leave compute units idle
+    int deep = 8;
+    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 1024) deep /= 2;
+    g.per = (int64_t)deep * nrl;
+    CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_bn_bwd: too many rows");
     const int ng = cdiv(rows, g.per);
-    CN_DISPATCH_DTYPE(dtype, T, {
-        if (signs) mx_bn_apply_kernel<T, true><<<dim3(ng, tiles), 256, 0, st>>>(g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
-        else mx_bn_apply_kernel<T, false><<<dim3(ng, tiles), 256, 0, st>>>(g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
-    });
+    MXBN_GO(mx_bn_apply_kernel, dim3(ng, tiles), g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
+#undef MXBN_GO
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     return CN_OK;
 }

@@ -5,29 +5,36 @@
 // (4 per block), which keeps every store of codes aligned and contiguous over the wave.
 #include "mx_common.h"
 
-template <typename T, int FMT, bool SIGNS>
+// U: chunks a thread has in flight; FULL: C is a multiple of 8
+template <typename T, int FMT, bool SIGNS, int U, bool FULL>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ x, const T* __restrict__ sg, uint8_t* __restrict__ codes,
                                                           uint8_t* __restrict__ scales, uint8_t* __restrict__ signs, int64_t chunks, int C,
-                                                          MxDiv cpr, int per) {
-    const int64_t base = (int64_t)blockIdx.x * (256 * per);
+                                                          MxDiv cpr) {
+    const int64_t base = (int64_t)blockIdx.x * (256 * U);
     const int64_t row0 = base / cpr.d;                                   // (uniform: one 64-bit division per workgroup)
     const uint32_t rem0 = (uint32_t)(base - row0 * cpr.d);
-    for (int u = 0; u < per; ++u) {
-        const uint32_t l = threadIdx.x + u * 256;
-        const int64_t i = base + l;
-        if (i >= chunks) return;                                         // (chunks is a multiple of 4: a quad stays whole)
-        const uint32_t n = rem0 + l, r = mx_quot(n, cpr);
+    MxRaw8<T> v[U], w[SIGNS ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t l = threadIdx.x + u * 256, n = rem0 + l, r = mx_quot(n, cpr);
         const int c0 = (int)(n - r * cpr.d) * 8;
         const int64_t at = (row0 + r) * C + c0;
-        float v[8];
-        mx_load8(x + at, C - c0, v);
-        const uint32_t b = mx_scale_byte<FMT>(quad_max_u(mx_absmax8(v)));
-        if (FMT == CN_MX_E2M1) reinterpret_cast<uint32_t*>(codes)[i] = mx_codes_e2m1(v, b);
-        else reinterpret_cast<uint2*>(codes)[i] = mx_codes_e4m3(v, b);
+        v[u].template load<FULL>(x, at, C - c0, base + l < chunks);
+        if (SIGNS) w[u].template load<FULL>(sg, at, C - c0, base + l < chunks);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t i = base + threadIdx.x + u * 256;
+        if (i >= chunks) return;                                         // (chunks is a multiple of 4: a quad stays whole)
+        float f[8];
+        v[u].get(f);
+        const uint32_t b = mx_scale_byte<FMT>(quad_max_u(mx_absmax8(f)));
+        if (FMT == CN_MX_E2M1) reinterpret_cast<uint32_t*>(codes)[i] = mx_codes_e2m1(f, b);
+        else reinterpret_cast<uint2*>(codes)[i] = mx_codes_e4m3(f, b);
         if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)b;
         if (SIGNS) {
             float s[8];
-            mx_load8(sg + at, C - c0, s);
+            w[u].get(s);
             uint32_t m = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j) m |= (s[j] > 0.f ? 1u : 0u) << j;
@@ -78,16 +85,19 @@ extern "C" int cn_mx_quantize(const void* x, void* codes, void* scales, const vo
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_quantize: codes must be 16-byte aligned");
     const uint32_t cpr = (uint32_t)cdiv(C, MX_BLOCK) * 4;
     const int64_t chunks = rows * cpr;
-    const int per = chunks >= (int64_t)256 * 4096 ? 4 : 1;
-    const int64_t grid = (chunks + 256 * per - 1) / (256 * per);
+    // four chunks a thread (64 or 128 bytes in flight) once that still leaves 16 workgroups a compute unit
+    const bool many = chunks >= (int64_t)256 * 4 * 4096, full = C % 8 == 0;
+    const int64_t grid = (chunks + 256 * (many ? 4 : 1) - 1) / (256 * (many ? 4 : 1));
     CN_CHECK_ARG(grid < ((int64_t)1 << 31), "cn_mx_quantize: tensor too large");
-#define MX_Q(FMT, SIGNS)                                                                                                               \
-    mx_quantize_kernel<T, FMT, SIGNS><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>((const T*)x, (const T*)sign_src, (uint8_t*)codes, \
-        (uint8_t*)scales, (uint8_t*)signs, chunks, C, mx_div(cpr), per)
+#define MX_Q(FMT, SIGNS, U, FULL)                                                                                                      \
+    mx_quantize_kernel<T, FMT, SIGNS, U, FULL><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>((const T*)x, (const T*)sign_src,       \
+        (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)signs, chunks, C, mx_div(cpr))
+#define MX_QU(FMT, SIGNS) do { if (many) { if (full) MX_Q(FMT, SIGNS, 4, true); else MX_Q(FMT, SIGNS, 4, false); } else { if (full) MX_Q(FMT, SIGNS, 1, true); else MX_Q(FMT, SIGNS, 1, false); } } while (0)
     CN_DISPATCH_DTYPE(dtype, T, {
-        if (fmt == CN_MX_E2M1) { if (signs) MX_Q(CN_MX_E2M1, true); else MX_Q(CN_MX_E2M1, false); }
-        else { if (signs) MX_Q(CN_MX_E4M3, true); else MX_Q(CN_MX_E4M3, false); }
+        if (fmt == CN_MX_E2M1) { if (signs) MX_QU(CN_MX_E2M1, true); else MX_QU(CN_MX_E2M1, false); }
+        else { if (signs) MX_QU(CN_MX_E4M3, true); else MX_QU(CN_MX_E4M3, false); }
     });
+#undef MX_QU
 #undef MX_Q
     CN_LAUNCH_CHECK("cn_mx_quantize");
     return CN_OK;

@@ -60,6 +60,14 @@ __device__ static inline void mx_put_dy(const MxRaw8<float>& r, bf16_t* lds, int
     *reinterpret_cast<u32x4_t*>(lds + 2 * plane) = pk(l);
 }
 
+template <typename R> __device__ static inline void mx_buf8(MxRaw8<bf16_t>& w, R rsrc, uint32_t ofs) {
+    w.a = __builtin_amdgcn_raw_buffer_load_b128(rsrc, ofs, 0, 0);
+}
+template <typename R> __device__ static inline void mx_buf8(MxRaw8<float>& w, R rsrc, uint32_t ofs) {
+    w.a = __builtin_amdgcn_raw_buffer_load_b128(rsrc, ofs, 0, 0);
+    w.b = __builtin_amdgcn_raw_buffer_load_b128(rsrc, ofs + 16, 0, 0);
+}
+
 template <typename T, int TN, int TK, bool FULL>
 __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     constexpr int NP = sizeof(T) == 2 ? 1 : 3;
@@ -84,47 +92,60 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     const int yleft = g.N - n0 - yc;
     const bool xok = k0 + xc < g.Kp;                              // (Kp is a multiple of 32: 16 codes are inside or outside)
 
-    MxRaw8<T> ry[YV];
-    uint4 rx[XV];
-    uint32_t rs[XV];
-    auto gload = [&](int64_t r0) {
+    // raw tiles on their way: two sets, so that a tile is asked for two tiles ahead of its use.  FULL (N a multiple of 8, dy on a 16-byte
+    // border): buffer loads whose range ends with the rows — what lies behind reads as zero, and the lanes' offsets are the same for
+    // every tile (columns behind the last: an offset out of range; offsets stay below 2^31 + 2^26, and all of one is in the lane's part:
+    // the range check subtracts a scalar part from the range, which wraps where that is the larger).
+    struct Raw { MxRaw8<T> y[YV]; u32x4_t x[XV]; uint32_t s[XV]; };
+    Raw ra;
+    constexpr uint32_t OUT = 0x80000000u;
+    const uint32_t yofs = yleft > 0 ? (uint32_t)(yr * g.N + n0 + yc) * sizeof(T) : OUT;
+    const uint32_t xofs = xok ? (uint32_t)(xr * g.Kp + k0 + xc) : OUT, sofs = xok ? (uint32_t)(xr * g.blocks + ((k0 + xc) >> 5)) : OUT;
+    auto gload = [&](Raw& w, int64_t r0) {
+        const int left = r0 < rend ? (rend - r0 < BR ? (int)(rend - r0) : BR) : 0;         // rows of this tile
+        const int64_t rr = left ? r0 : rbeg;
+        if (FULL) {
+            const auto by = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(reinterpret_cast<const T*>(g.dy) + rr * g.N), 0, (uint32_t)left * g.N * sizeof(T), 0x00020000);
 #pragma unroll
-        for (int v = 0; v < YV; ++v) {
-            const int64_t r = r0 + yr + v * (256 / YC);
-            ry[v].template load<FULL>(reinterpret_cast<const T*>(g.dy), r * g.N + n0 + yc, yleft, r < rend);
+            for (int v = 0; v < YV; ++v) mx_buf8(w.y[v], by, yofs + (uint32_t)(v * (256 / YC)) * g.N * sizeof(T));
+        } else {
+#pragma unroll
+            for (int v = 0; v < YV; ++v) {
+                const int r = yr + v * (256 / YC);
+                w.y[v].template load<false>(reinterpret_cast<const T*>(g.dy), (rr + r) * g.N + n0 + yc, yleft, r < left);
+            }
         }
+        const auto bx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.codes + rr * g.Kp), 0, (uint32_t)left * g.Kp, 0x00020000);
+        const auto bs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.scales + rr * g.blocks), 0, (uint32_t)left * g.blocks, 0x00020000);
 #pragma unroll
         for (int v = 0; v < XV; ++v) {
-            const int64_t r = r0 + xr + v * (256 / XC);
-            const bool ok = xok && r < rend;
-            rx[v] = ldg16_masked(g.codes, r * g.Kp + k0 + xc, ok);
-            rs[v] = g.scales[ok ? r * g.blocks + ((k0 + xc) >> 5) : 0];
-            rs[v] = ok ? rs[v] : 127u;                            // (codes are zero there: any finite scale)
+            w.x[v] = __builtin_amdgcn_raw_buffer_load_b128(bx, xofs + (uint32_t)(v * (256 / XC)) * g.Kp, 0, 0);
+            w.s[v] = __builtin_amdgcn_raw_buffer_load_b8(bs, sofs + (uint32_t)(v * (256 / XC)) * g.blocks, 0, 0);
         }
     };
     float sb[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sb[j] = 0.f;
-    auto lstore = [&]() {
+    auto lstore = [&](const Raw& w) {
 #pragma unroll
         for (int v = 0; v < YV; ++v) {
-            mx_put_dy(ry[v], ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
+            mx_put_dy(w.y[v], ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
             if (bias) {
                 float f[8];
-                ry[v].get(f);
+                w.y[v].get(f);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sb[j] += f[j];
             }
         }
 #pragma unroll
         for (int v = 0; v < XV; ++v) {
-            const float s = mx_scale_value(rs[v]);
-            const uint32_t w[4] = {rx[v].x, rx[v].y, rx[v].z, rx[v].w};
+            const float s = mx_scale_value(w.s[v]);
+            const uint32_t q[4] = {w.x[v].x, w.x[v].y, w.x[v].z, w.x[v].w};
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, false));
-                o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], s, true));
+                o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], s, false));
+                o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], s, true));
             }
             bf16_t* p = lx + (xr + v * (256 / XC)) * XP + xc;
             st16(p, make_uint4(o[0], o[1], o[2], o[3]));
@@ -140,12 +161,11 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-    gload(rbeg);
-    for (int64_t r0 = rbeg; r0 < rend; r0 += BR) {
+    auto tile = [&](Raw& w, int64_t r0) {
         __syncthreads();                                          // the previous tile has been read
-        lstore();
+        lstore(w);
         __syncthreads();
-        if (r0 + BR < rend) gload(r0 + BR);
+        gload(w, r0 + BR);                                        // (behind the end: zeros)
 #pragma unroll
         for (int s = 0; s < BR / 16; ++s) {
             bf16x8_t b[NJ];
@@ -160,7 +180,9 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
                     for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
                 }
         }
-    }
+    };
+    gload(ra, rbeg);
+    for (int64_t r0 = rbeg; r0 < rend; r0 += BR) tile(ra, r0);
 
     float* dw = g.dw + (int64_t)blockIdx.x * g.N * g.K;
 #pragma unroll
@@ -192,30 +214,62 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     }
 }
 
-// out[i] = (accumulate ? out[i] : 0) + sum_s part[s][i], the splits in order
+// out[i] = (accumulate ? out[i] : 0) + sum_s part[s][i] for i < n (dw) and then n <= i < n + nb (db).  GS split groups of 256 / GS threads,
+// four outputs a thread; the groups meet in LDS in order.
+template <int GS>
 __global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int splits,
                                                             const float* __restrict__ part_b, float* __restrict__ out_b, int nb, int accumulate) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n + nb) return;
-    const bool w = i < n;
-    const float* p = w ? part + i : part_b + (i - n);
-    const int64_t step = w ? n : nb;
-    float s = 0.f;
+    constexpr int TO = 256 / GS;
+    __shared__ float red[GS][TO * 4];
+    const int o = threadIdx.x % TO, gs = threadIdx.x / TO;
+    const int64_t wgs_w = (n + TO * 4 - 1) / (TO * 4);             // workgroups of dw come first
+    const bool w = blockIdx.x < wgs_w;
+    const int64_t len = w ? n : nb, i0 = ((int64_t)blockIdx.x - (w ? 0 : wgs_w)) * (TO * 4) + o * 4;
+    const float* p = (w ? part : part_b) + i0;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i0 + 4 <= len) {
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += p[(int64_t)k * step];
-    float* o = w ? out + i : out_b + (i - n);
-    *o = accumulate ? *o + s : s;
+        for (int k = gs; k < splits; k += GS) {
+            const u32x4_t v = *reinterpret_cast<const u32x4_a4*>(p + k * len);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += __uint_as_float(v[j]);
+        }
+    } else {
+        for (int k = gs; k < splits; k += GS)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += i0 + j < len ? p[k * len + j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[gs][o * 4 + j] = s[j];
+    __syncthreads();
+    for (int t = threadIdx.x; t < TO * 4; t += 256) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < GS; ++k) v += red[k][t];
+        const int64_t i = i0 - o * 4 + t;
+        if (i < len) {
+            float* q = (w ? out : out_b) + i;
+            *q = accumulate ? *q + v : v;
+        }
+    }
 }
 
-struct MxWgPlan { int tn, tk, ntiles, ktiles, splits; int64_t per; };
+// Tiles and splits.  Large problems take the wide tiles (a row of dy / x8 is read again for every K / N tile) and two workgroups a compute
+// unit; small ones the narrow tiles, whose workgroups are short of work sooner, and no split once the tiles alone fill the card (each
+// split writes and reads a whole dw).  us, wide | narrow, bf16: 262144x256x128 43 | 66, 65536x1024x256 54 | 93, 16384x512x2048 55 | 96;
+// 8192x512x512 24.2 | 21.5, 65536x256x64 18.3 | 15.2, 4096x1024x256 18.9 | 15.9, 1024x2048x512 14.0 | 11.8 (15.1 in two splits).
+// 32 bits (64 x 128 | 64 x 64): 65536x1024x256 139 | 199, 65536x256x64 19.8 | 21.5, 30000x80x208 20.2 | 23.5; 512x256x256 9.0 | 8.1.
+struct MxWgPlan { bool wide; int tn, tk, ntiles, ktiles, splits; int64_t per; };
 static MxWgPlan mxwg_plan(int64_t rows, int K, int N, int dtype) {
     MxWgPlan p;
-    p.tn = (N > 64 && dtype == CN_BF16) ? 128 : 64;
-    p.tk = K > 64 ? 128 : 64;
+    const double macs = (double)rows * K * N;
+    p.wide = dtype == CN_BF16 ? (macs >= 4e9 && N > 64 && K > 64) : (macs >= 4e8 && K > 64);
+    p.tn = p.wide && dtype == CN_BF16 ? 128 : 64;
+    p.tk = p.wide ? 128 : 64;
     p.ntiles = cdiv(N, p.tn);
     p.ktiles = cdiv(K, p.tk);
     const int64_t tiles = (int64_t)p.ntiles * p.ktiles, rtiles = (rows + 63) / 64;
-    int64_t s = 768 / tiles;                      // three workgroups a CU
+    int64_t s = tiles >= 192 ? 1 : 512 / tiles;
     s = s < rtiles ? s : rtiles;
     s = s < 1 ? 1 : s;
     p.per = (rtiles + s - 1) / s * 64;
@@ -232,7 +286,7 @@ extern "C" size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype
 template <typename T, int TN, int TK>
 static void mxwg_launch(const MxWgGeom& g, const MxWgPlan& p, hipStream_t st) {
     const dim3 grid(p.splits, p.ntiles * p.ktiles);
-    if (g.N % 8 == 0) mx_wgrad_kernel<T, TN, TK, true><<<grid, 256, 0, st>>>(g);
+    if (g.N % 8 == 0 && ((uintptr_t)g.dy & 15) == 0) mx_wgrad_kernel<T, TN, TK, true><<<grid, 256, 0, st>>>(g);
     else mx_wgrad_kernel<T, TN, TK, false><<<grid, 256, 0, st>>>(g);
 }
 
@@ -266,19 +320,19 @@ extern "C" int cn_mx_linear_wgrad(const void* dy, const void* codes, const void*
     g.ktiles = p.ktiles;
     g.accumulate = join ? 0 : accumulate;
     if (dtype == CN_BF16) {
-        if (p.tn == 128 && p.tk == 128) mxwg_launch<bf16_t, 128, 128>(g, p, st);
-        else if (p.tn == 128) mxwg_launch<bf16_t, 128, 64>(g, p, st);
-        else if (p.tk == 128) mxwg_launch<bf16_t, 64, 128>(g, p, st);
+        if (p.wide) mxwg_launch<bf16_t, 128, 128>(g, p, st);
         else mxwg_launch<bf16_t, 64, 64>(g, p, st);
     } else {
-        if (p.tk == 128) mxwg_launch<float, 64, 128>(g, p, st);
+        if (p.wide) mxwg_launch<float, 64, 128>(g, p, st);
         else mxwg_launch<float, 64, 64>(g, p, st);
     }
     CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
     if (join) {
         const int64_t n = (int64_t)N * K;
         const int nb = db ? N : 0;
-        mx_wgrad_join_kernel<<<(unsigned)((n + nb + 255) / 256), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        // sixteen groups where the splits are many and the outputs few; 64 / 1024 outputs a workgroup
+        if (p.splits >= 16) mx_wgrad_join_kernel<16><<<(unsigned)(cdiv(n, 64) + cdiv(nb, 64)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        else mx_wgrad_join_kernel<1><<<(unsigned)(cdiv(n, 1024) + cdiv(nb, 1024)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
     }
     return CN_OK;
