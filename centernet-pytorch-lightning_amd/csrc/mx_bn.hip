@@ -90,42 +90,39 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
     }
 }
 
-// 16 channels x 64 partial rows per workgroup: totals, parameter gradients, and the coefficients a, b, c of dx
+// Four channels a workgroup, a thread per partial row: totals, parameter gradients, and the coefficients a, b, c of dx.  The partial sums
+// were written from all over the card: few workgroups with long chains of such reads cost 19 us for 1024 x 256 channels, this 7 us.
 __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, float inv_rows,
                                                            const float* __restrict__ gamma, const float* __restrict__ invstd,
                                                            float* __restrict__ coef, float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                            int accumulate) {
-    __shared__ float red[64][2][17];
-    const int cl = (threadIdx.x & 3) * 4, gl = threadIdx.x >> 2, c0 = blockIdx.x * 16;
-    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    int at[4];                                                     // (channels behind the last read the last one's sums; they are dropped)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) at[j] = c0 + cl + j < C ? c0 + cl + j : C - 1;
+    __shared__ float red[4][8];
+    const int tid = threadIdx.x, c0 = blockIdx.x * 4;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};       // sums of d, of d (x8 - mean), four channels each
+    if (c0 + 4 <= C) {
 #pragma unroll 4
-    for (int g = gl; g < groups; g += 64) {
-        const float* p = part + (int64_t)g * 2 * C;
+        for (int g = tid; g < groups; g += 256) {
+            const float* p = part + (int64_t)g * 2 * C + c0;
+            const u32x4_t a = *reinterpret_cast<const u32x4_a4*>(p), b = *reinterpret_cast<const u32x4_a4*>(p + C);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { s[0][j] += p[at[j]]; s[1][j] += p[C + at[j]]; }
+            for (int j = 0; j < 4; ++j) { s[j] += __uint_as_float(a[j]); s[4 + j] += __uint_as_float(b[j]); }
+        }
+    } else {
+        for (int g = tid; g < groups; g += 256)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c0 + j < C) { s[j] += part[(int64_t)g * 2 * C + c0 + j]; s[4 + j] += part[((int64_t)g * 2 + 1) * C + c0 + j]; }
     }
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int j = 0; j < 8; ++j) s[j] = wave_sum(s[j]);
+    if ((tid & 63) == 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) red[gl][k][cl + j] = s[k][j];
+        for (int j = 0; j < 8; ++j) red[tid >> 6][j] = s[j];
     __syncthreads();
-    // 32 totals, eight threads each
-    const int o = threadIdx.x >> 3, q = threadIdx.x & 7, k = o >> 4, cc = o & 15;
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += red[q * 8 + i][k][cc];
-    t += __shfl_xor(t, 1, 64);
-    t += __shfl_xor(t, 2, 64);
-    t += __shfl_xor(t, 4, 64);
-    __syncthreads();
-    if (q == 0) red[0][k][cc] = t;
-    __syncthreads();
-    const int ch = c0 + threadIdx.x;
-    if (threadIdx.x < 16 && ch < C) {
-        const float s0 = red[0][0][threadIdx.x], s1 = red[0][1][threadIdx.x];
+    const int ch = c0 + tid;
+    if (tid < 4 && ch < C) {
+        const float s0 = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+        const float s1 = (red[0][4 + tid] + red[1][4 + tid]) + (red[2][4 + tid] + red[3][4 + tid]);
         const float is = invstd[ch], dg = s1 * is, a = gamma[ch] * is;
         coef[ch] = a;
         coef[C + ch] = a * is * dg * inv_rows;
@@ -135,24 +132,61 @@ __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restri
     }
 }
 
-template <typename T, bool SIGNS, bool FULL>
-__global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, const float* __restrict__ mean, const float* __restrict__ coef,
+// what the finish pass leaves, or what the apply pass needs to do its work itself (few groups: a launch costs more than the repeated sums)
+struct MxBnTail {
+    const float* coef;
+    const float* part;
+    const float* gamma;
+    const float* invstd;
+    float* dgamma;
+    float* dbeta;
+    float inv_rows;
+    int groups, accumulate;
+};
+
+template <typename T, bool SIGNS, bool FULL, bool JOIN>
+__global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, const float* __restrict__ mean, const MxBnTail t,
                                                           T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc) {
     const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
     const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
     if (left <= 0) return;
     const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
     float ka[8], kb[8], kc[8], mu[8];
-    {
+    auto get = [&](const float* p, float (&o)[8]) {
         MxRaw8<float> k;
-        k.template load<FULL>(coef, c * 8, left, true);
-        k.get(ka);
-        k.template load<FULL>(coef, g.C + c * 8, left, true);
-        k.get(kb);
-        k.template load<FULL>(coef, 2 * g.C + c * 8, left, true);
-        k.get(kc);
-        k.template load<FULL>(mean, c * 8, left, true);
-        k.get(mu);
+        k.template load<FULL>(p, c * 8, left, true);
+        k.get(o);
+    };
+    get(mean, mu);
+    if (JOIN) {
+        float s0[8], s1[8], is[8], ga[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; }
+#pragma unroll 4
+        for (int k = 0; k < t.groups; ++k) {
+            float a[8], b[8];
+            get(t.part + (int64_t)k * 2 * g.C, a);
+            get(t.part + ((int64_t)k * 2 + 1) * g.C, b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { s0[j] += a[j]; s1[j] += b[j]; }
+        }
+        get(t.invstd, is);
+        get(t.gamma, ga);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float dg = s1[j] * is[j];
+            ka[j] = ga[j] * is[j];
+            kb[j] = ka[j] * is[j] * dg * t.inv_rows;
+            kc[j] = ka[j] * s0[j] * t.inv_rows;
+            if (blockIdx.x == 0 && rl == 0 && j < left) {
+                t.dgamma[c * 8 + j] = t.accumulate ? t.dgamma[c * 8 + j] + dg : dg;
+                t.dbeta[c * 8 + j] = t.accumulate ? t.dbeta[c * 8 + j] + s0[j] : s0[j];
+            }
+        }
+    } else {
+        get(t.coef, ka);
+        get(t.coef + g.C, kb);
+        get(t.coef + 2 * g.C, kc);
     }
     for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
         MxBnRow<T> row[MXBN_U];
@@ -186,10 +220,11 @@ static int mxbn_lg(int C) {
     while (lg < 5 && (1 << lg) < chunks) ++lg;
     return lg;
 }
-// row groups of the sums pass: ~1024 workgroups in all, at least two rows for a thread
+#define MXBN_JOIN 32           // row groups up to which the apply pass adds the partial sums up itself
+// row groups of the sums pass: ~1024 workgroups in all, at least four rows for a thread
 static int mxbn_groups(int64_t rows, int C) {
     const int lg = mxbn_lg(C), tiles = cdiv(cdiv(C, 8), 1 << lg);
-    const int64_t most = (rows + 2 * (256 >> lg) - 1) / (2 * (256 >> lg));
+    const int64_t most = (rows + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
     int64_t g = 1024 / tiles;
     g = g < most ? g : most;
     return (int)(g < 1 ? 1 : (g > MXBN_MAX_GROUPS ? MXBN_MAX_GROUPS : g));
@@ -222,23 +257,30 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
     g.per = (rows + groups - 1) / groups;
     const bool full = C % 8 == 0;
-#define MXBN_GO(KERNEL, GRID, ...)                                                                                                     \
+#define MXBN_GO(KERNEL, MORE, GRID, ...)                                                                                               \
     CN_DISPATCH_DTYPE(dtype, T, {                                                                                                      \
-        if (signs) { if (full) KERNEL<T, true, true><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, true, false><<<GRID, 256, 0, st>>>(__VA_ARGS__); }      \
-        else { if (full) KERNEL<T, false, true><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, false, false><<<GRID, 256, 0, st>>>(__VA_ARGS__); }          \
+        if (signs) { if (full) KERNEL<T, true, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, true, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }  \
+        else { if (full) KERNEL<T, false, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, false, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }      \
     })
-    MXBN_GO(mx_bn_sums_kernel, dim3(groups, tiles), g, mean, part);
+#define MXBN_COMMA ,
+    MXBN_GO(mx_bn_sums_kernel, , dim3(groups, tiles), g, mean, part);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
-    mx_bn_finish_kernel<<<cdiv(C, 16), 256, 0, st>>>(part, groups, C, 1.f / (float)rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
-    CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    const MxBnTail t{coef, part, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, groups, accumulate};
+    const bool joined = groups <= MXBN_JOIN;
+    if (!joined) {
+        mx_bn_finish_kernel<<<cdiv(C, 4), 256, 0, st>>>(part, groups, C, t.inv_rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
+        CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    }
     // eight rows a thread (its coefficients are loaded once), fewer where that would leave compute units idle
     int deep = 8;
     while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 1024) deep /= 2;
     g.per = (int64_t)deep * nrl;
     CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_bn_bwd: too many rows");
     const int ng = cdiv(rows, g.per);
-    MXBN_GO(mx_bn_apply_kernel, dim3(ng, tiles), g, mean, coef, (T*)dx, (T*)dres, (const T*)racc);
+    if (joined) MXBN_GO(mx_bn_apply_kernel, MXBN_COMMA true, dim3(ng, tiles), g, mean, t, (T*)dx, (T*)dres, (const T*)racc);
+    else MXBN_GO(mx_bn_apply_kernel, MXBN_COMMA false, dim3(ng, tiles), g, mean, t, (T*)dx, (T*)dres, (const T*)racc);
 #undef MXBN_GO
+#undef MXBN_COMMA
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     return CN_OK;
 }

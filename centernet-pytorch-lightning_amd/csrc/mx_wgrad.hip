@@ -76,6 +76,7 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     constexpr int YV = BR * TN / 8 / 256, XV = BR * TK / 16 / 256;
     constexpr int YC = TN / 8, XC = TK / 16;
     constexpr int MI = TN / 64, NJ = TK / 64;                     // 2 x 2 waves of 32 x 32 tiles
+    constexpr int DEEP = TN * TK == 64 * 64 ? 2 : 1;              // tiles in flight: the wide tiles have no registers for a second
     constexpr int PLANE = BR * YP;
     __shared__ __attribute__((aligned(16))) bf16_t lds[NP * PLANE + BR * XP];
     bf16_t* const ly = lds;
@@ -92,12 +93,12 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     const int yleft = g.N - n0 - yc;
     const bool xok = k0 + xc < g.Kp;                              // (Kp is a multiple of 32: 16 codes are inside or outside)
 
-    // raw tiles on their way: two sets, so that a tile is asked for two tiles ahead of its use.  FULL (N a multiple of 8, dy on a 16-byte
+    // raw tiles on their way, asked for DEEP tiles ahead of their use.  FULL (N a multiple of 8, dy on a 16-byte
     // border): buffer loads whose range ends with the rows — what lies behind reads as zero, and the lanes' offsets are the same for
     // every tile (columns behind the last: an offset out of range; offsets stay below 2^31 + 2^26, and all of one is in the lane's part:
     // the range check subtracts a scalar part from the range, which wraps where that is the larger).
     struct Raw { MxRaw8<T> y[YV]; u32x4_t x[XV]; uint32_t s[XV]; };
-    Raw ra;
+    Raw ra, rb;
     constexpr uint32_t OUT = 0x80000000u;
     const uint32_t yofs = yleft > 0 ? (uint32_t)(yr * g.N + n0 + yc) * sizeof(T) : OUT;
     const uint32_t xofs = xok ? (uint32_t)(xr * g.Kp + k0 + xc) : OUT, sofs = xok ? (uint32_t)(xr * g.blocks + ((k0 + xc) >> 5)) : OUT;
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
         __syncthreads();                                          // the previous tile has been read
         lstore(w);
         __syncthreads();
-        gload(w, r0 + BR);                                        // (behind the end: zeros)
+        gload(w, r0 + DEEP * BR);                                 // (behind the end: zeros)
 #pragma unroll
         for (int s = 0; s < BR / 16; ++s) {
             bf16x8_t b[NJ];
@@ -182,7 +183,15 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
         }
     };
     gload(ra, rbeg);
-    for (int64_t r0 = rbeg; r0 < rend; r0 += BR) tile(ra, r0);
+    if (DEEP == 1) {
+        for (int64_t r0 = rbeg; r0 < rend; r0 += BR) tile(ra, r0);
+    } else {
+        gload(rb, rbeg + BR);
+        for (int64_t r0 = rbeg; r0 < rend; r0 += 2 * BR) {
+            tile(ra, r0);
+            if (r0 + BR < rend) tile(rb, r0 + BR);
+        }
+    }
 
     float* dw = g.dw + (int64_t)blockIdx.x * g.N * g.K;
 #pragma unroll
