@@ -31,12 +31,27 @@ class MXTensor:
     `shape` and `dtype` it was made from, and optionally `signs` uint8 [rows, Cp / 8] (see `checkpoint`) — three views of one buffer."""
     __slots__ = ("buffer", "shape", "dtype", "fmt", "rows", "blocks", "has_signs", "_n")
 
-    def __init__(self, shape, dtype, fmt, device, signs=False):
+    def __init__(self, shape, dtype, fmt, device, signs=False, buffer=None):
         self.shape, self.dtype, self.fmt, self.has_signs = shape, dtype, fmt, signs
         self.blocks = (shape[-1] + BLOCK - 1) // BLOCK
         self.rows = shape[:-1].numel()
         self._n = self.rows * self.blocks                  # blocks in all
-        self.buffer = torch.empty(self._n * ((33 if fmt == "e4m3" else 17) + (4 if signs else 0)), dtype=torch.uint8, device=device)
+        n = self._n * ((33 if fmt == "e4m3" else 17) + (4 if signs else 0))
+        if buffer is None:
+            buffer = torch.empty(n, dtype=torch.uint8, device=device)
+        elif buffer.numel() != n:
+            raise ValueError(f"MXTensor: a buffer of {n} bytes is needed, got {buffer.numel()}")
+        self.buffer = buffer
+
+    @property
+    def meta(self):
+        """what makes the tensor again from its buffer: `MXTensor.of(buffer, meta)` (an autograd node saves the buffer)"""
+        return self.shape, self.dtype, self.fmt, self.has_signs
+
+    @classmethod
+    def of(cls, buffer, meta):
+        shape, dtype, fmt, signs = meta
+        return cls(shape, dtype, fmt, buffer.device, signs, buffer)
 
     def _pointers(self):
         """codes, scales, signs (None without)"""

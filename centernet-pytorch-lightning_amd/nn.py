@@ -13,7 +13,7 @@ import torch.nn as nn
 
 import os
 
-from . import ops
+from . import mx, ops
 
 STEM_BN_FUSED = not (os.environ.get("CN_DISABLE_STEM_BN_FUSED") or os.environ.get("CN_DISABLE_WGRAD_C16"))   # stem conv + BN as one autograd node
 # training-mode BN of the 16-channel 512^2 layers applied by the consuming conv: needs the kernels with the pre-affine hook, so the
@@ -22,6 +22,9 @@ BN_DEFER = not (os.environ.get("CN_DISABLE_BN_DEFER") or os.environ.get("CN_DISA
 
 
 class Conv2d(nn.Module):
+    ckpt8 = False           # `use_checkpoints`: keep the input in 8 bits for the backward pass
+    mx4 = False             # `use_mxfp4`: the no-grad forward as a 4-bit product (1x1, stride 1)
+
     def __init__(self, cin, cout, k, stride=1, padding=0, bias=False):
         super().__init__()
         self.stride, self.padding, self.k = stride, padding, k
@@ -42,6 +45,8 @@ class Conv2d(nn.Module):
         """bn_stats: the output goes straight into a training-mode BatchNorm2d (ops.BnStats: statistics from the conv epilogue)"""
         pre = getattr(x, "_cn_pre", None)           # x is a raw conv output whose BN (+ ReLU) is applied by this conv's kernels (ops.BnDeferFn)
         if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad):
+            if self.ckpt8 and pre is None and not (relu or mask_dx or defer_relu_bwd):
+                return ops.conv2d_ckpt(x, self.weight, self.bias, self.stride, self.padding, bn_stats)
             return ops.conv2d(x, self.weight, self.bias, self.stride, self.padding, relu, mask_dx, defer_relu_bwd, bn_stats=bn_stats, pre=pre)
         if pre is not None:
             c = self.infer_key(x)
@@ -54,9 +59,9 @@ class Conv2d(nn.Module):
     def with_skip(self, x, bn_stats=False):
         """-> (conv(x), x) for a residual connection around this conv: the skip path's gradient is added in the epilogue of this
         conv's data-gradient kernel (training; otherwise just the pair)."""
-        if torch.is_grad_enabled() and x.requires_grad and self.stride == 1:
+        if torch.is_grad_enabled() and x.requires_grad and self.stride == 1 and not self.ckpt8:
             return ops.conv2d(x, self.weight, self.bias, self.stride, self.padding, False, False, False, True, bn_stats=bn_stats)
-        return self.forward(x), x
+        return self.forward(x, bn_stats=bn_stats), x
 
     def infer_key(self, x, scale=None, shift=None):
         """-> the cache entry {wp: packed (folded) weights, b: folded bias} for x's dtype and the current parameter versions"""
@@ -73,20 +78,49 @@ class Conv2d(nn.Module):
 
     def infer(self, x, scale, shift, residual, relu, out_dtype=None):
         """No-grad path: y = act(conv(x)*scale + shift + residual); packed (folded) weights are cached."""
+        if self.mx4 and out_dtype in (None, x.dtype):
+            w, b = self._mx_weight(x, scale, shift)
+            return mx.linear(x, w, b, residual, relu)
         c = self.infer_key(x, scale, shift)
         Co, _, KH, KW = self.weight.shape
         N, H, W, _ = x.shape
         OH, OW = ops.conv_out(H, KH, self.stride, self.padding), ops.conv_out(W, KW, self.stride, self.padding)
         return ops._igemm(x, c["wp"], c["b"], residual, Co, KH, KW, self.stride, self.padding, False, relu, OH, OW, out_dtype)
 
+    def _mx_weight(self, x, scale, shift):
+        """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels; kept per
+        weight version like `infer_key`'s"""
+        key = (x.shape[-1], x.device, self.weight._version, None if self.bias is None else self.bias._version, ops.WeightsEpoch.value,
+               None if scale is None else (scale.data_ptr(), scale._version))
+        hit = self.__dict__.get("_mx_cache")
+        if hit is None or hit[0] != key:
+            Co, Ci = self.weight.shape[:2]
+            with torch.no_grad():
+                w = torch.zeros(ops.rup(Co, 16), x.shape[-1], dtype=torch.float32, device=x.device)
+                w[:Co, :Ci] = self.weight.view(Co, Ci) if scale is None else self.weight.view(Co, Ci) * scale[:, None]
+                b = torch.zeros(w.shape[0], dtype=torch.float32, device=x.device)
+                if self.bias is not None:
+                    b[:Co] = self.bias if scale is None else self.bias * scale
+                if shift is not None:
+                    b[:Co] += shift
+            hit = self._mx_cache = (key, mx.pack_weight(w), b)
+        return hit[1], hit[2]
+
     def infer_nchw(self, x):
         """No-grad 1x1 conv + bias straight into the public fp32 NCHW layout (a head's last layer); packed weights cached as in `infer`."""
+        if self.mx4:
+            y = self.infer(x, None, None, None, False)
+            N, H, W, ld = y.shape
+            out = torch.empty((N, self.weight.shape[0], H, W), dtype=torch.float32, device=x.device)
+            ops.call("cn_nhwc_to_nchw", y, out, N, self.weight.shape[0], H, W, ld, ops.dtype_code(y.dtype))
+            return out
         self.infer_key(x)
         return ops.conv1x1_to_nchw(x, self._cache["wp"], self._cache["b"], self.weight.shape[0])
 
 
 class BatchNorm2d(nn.BatchNorm2d):
     """Parameter/buffer holder with nn.BatchNorm2d's state_dict; the arithmetic lives in ops.BatchNormActFn."""
+    ckpt8 = False           # `use_checkpoints`: keep the input in 8 bits for the backward pass
 
     def __init__(self, c):
         super().__init__(c, momentum=ops.BN_MOMENTUM)
@@ -117,6 +151,8 @@ class BatchNorm2d(nn.BatchNorm2d):
         if self.training:
             self._pending += 1
             ops.WeightsEpoch.bump()              # running_mean / running_var are about to change through raw pointers
+            if self.ckpt8 and torch.is_grad_enabled():
+                return ops.batch_norm_act(x, self, residual, relu, ckpt=True)
             if (defer and BN_DEFER and residual is None and x.dtype == torch.bfloat16 and x.shape[-1] == 16
                     and getattr(x, "_bn_part", None) is not None and getattr(x, "_cn_pre", None) is None):
                 return ops.batch_norm_defer(x, self, relu)
@@ -142,8 +178,10 @@ def cat_conv_bn_act(conv, bn, xs, residual=None, relu=True):
         return conv_bn_act(conv, bn, ops.concat(list(xs)), residual, relu)
     grad = torch.is_grad_enabled() and (conv.weight.requires_grad or any(t.requires_grad for t in xs))
     if bn.training or grad:
-        return bn(ops.conv1x1_cat(xs, conv.weight, bn_stats=bn.training), residual, relu)
+        return bn(ops.conv1x1_cat(xs, conv.weight, bn_stats=bn.training, ckpt=conv.ckpt8), residual, relu)
     s, b = bn.folded()                              # eval: BN folded into the packed weights, one launch
+    if conv.mx4:
+        return conv.infer(ops.concat(list(xs)), s, b, residual, relu)
     key = ("cat", xs[0].dtype, conv.weight._version, ops.WeightsEpoch.value, s.data_ptr(), s._version)
     if conv._cache.get("k") != key:
         conv._cache = {"k": key, "wp": ops.pack_weight(conv.weight, 1, xs[0].dtype, s), "b": b}
@@ -181,7 +219,7 @@ class StemConv(nn.Module):
 
 def stem_bn_act(stem, bn, img, dtype, relu=True, defer=False):
     """stem conv -> BN -> ReLU; one fused kernel in eval / no-grad mode.  defer: see BatchNorm2d.forward."""
-    if (defer and BN_DEFER and STEM_BN_FUSED and bn.training and dtype == torch.bfloat16 and stem.weight.shape[0] == 16
+    if (defer and BN_DEFER and STEM_BN_FUSED and bn.training and not bn.ckpt8 and dtype == torch.bfloat16 and stem.weight.shape[0] == 16
             and stem.weight.shape[2] == 7 and stem.padding == 3 and stem.weight.shape[1] <= 3 and ops.BnStats.enabled):
         # the BN behind the stem lives entirely in the neighbouring kernels (ops.StemBnDeferFn)
         bn._pending += 1
@@ -265,3 +303,27 @@ class MaxPool2d(nn.Module):
 
     def forward(self, x):
         return ops.max_pool(x, self.k, self.stride, self.padding)
+
+
+def use_checkpoints(module, on=True):
+    """Training with 8-bit activation checkpoints: every Conv2d and BatchNorm2d under `module` keeps its input in e4m3 (one scale per 32
+    channels) and a ReLU's mask in bits, instead of the bf16 / fp32 tensors.  The forward pass is unchanged; gradients are those of
+    the layers at the rounded inputs.  (The task heads, DCN and transposed convolutions keep what they kept.)  -> layers switched"""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, (Conv2d, BatchNorm2d)):
+            m.ckpt8 = bool(on)
+            n += 1
+    return n
+
+
+def use_mxfp4(module, on=True):
+    """No-grad forward with 4-bit products: every 1x1 / stride-1 Conv2d under `module` quantises its input and its (BN-folded) weights to
+    e2m1 with one scale per 32 channels (mx.linear).  Training is not affected.  Pass the whole model or only its backbone: a head's
+    last convolution is a 1x1 too.  -> layers switched"""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, Conv2d) and m.k == 1 and m.stride == 1 and m.padding == 0:
+            m.mx4 = bool(on)
+            n += 1
+    return n

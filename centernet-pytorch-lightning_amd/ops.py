@@ -7,7 +7,7 @@ reference.  Every op enqueues hand-written HIP kernels on the current stream thr
 import torch
 from torch.autograd import Function
 
-from . import _hip
+from . import _hip, mx
 from ._hip import Hooks, call, dtype_code
 
 import os as _os
@@ -297,12 +297,13 @@ class GradCell:
     content to the producer.  A consumer without an epilogue slot (DCNv2's sampling gradient, a pass-through residual) that finds
     the cell occupied pays one cn_add; consumers that know nothing about cells return their gradient as usual and are summed in
     `ShareFn.backward` — the result is the same sum in every case (bf16 rounding of partial sums as with autograd's own adds)."""
-    __slots__ = ("partial", "sparse")
+    __slots__ = ("partial", "sparse", "ck")
     enabled = not _os.environ.get("CN_DISABLE_GRAD_CELLS")
     adds = 0            # cn_add launches spent on cells (tests / profiling)
 
     def __init__(self):
         self.partial = None
+        self.ck = None        # (version, e4m3 checkpoint) of the tensor, for the consumers that keep one (_input_checkpoint)
         self.sparse = []      # closures fn(total) that scatter-add a consumer's few non-zero gradient rows into the finished sum (HeadFn)
 
     def take(self, like=None):
@@ -349,6 +350,7 @@ class ShareFn(Function):
     @staticmethod
     def backward(ctx, g):
         total = ctx.cell.take()
+        ctx.cell.ck = None
         if g is not None:
             total = g if total is None else _add_tensors(total, g)
         if ctx.cell.sparse:
@@ -752,6 +754,78 @@ def _conv2d_bwd(x, weight, bias_ref, dy, stride, pad, has_bias, mask_dx, cell, o
     return dx, dw, db
 
 
+def _input_checkpoint(x):
+    """x's e4m3 checkpoint.  The layers that read one shared tensor keep one between them: it lies in the tensor's GradCell, which `share`
+    makes anew in every forward pass."""
+    cell = cell_of(x)
+    if cell is None:
+        return mx.checkpoint(x)
+    if cell.ck is None or cell.ck[0] != x._version:
+        cell.ck = (x._version, mx.checkpoint(x))
+    return cell.ck[1]
+
+
+def _shape_only(ck):
+    """a tensor with the checkpointed input's shape and type and no memory, for code that reads nothing else of it"""
+    return torch.empty((1,) * len(ck.shape), dtype=ck.dtype, device=ck.device).expand(ck.shape)
+
+
+def _ckpt_wgrad(dy, ck, weight, bias, order):
+    """Weight (+ bias) gradient of a 1x1 convolution from its input's checkpoint: -> (dw, db), or (None, None) when they were deposited
+    in `.grad` on the side stream (inside a TrainStep)"""
+    Co = weight.shape[0]
+    if dy.shape[-1] != Co:
+        dy = dy[..., :Co].contiguous()
+    if SideGrads.usable(weight, bias):
+        def side_work():
+            mx.linear_wgrad(dy, ck, into=weight.grad, bias=bias is not None, bias_into=None if bias is None else bias.grad)
+            GradReady.note(weight, bias)
+        SideGrads.submit(SideGrads.wide_if_tail(side_work, order), dy, ck.buffer, claims=(weight, bias))
+        return None, None
+    dw, db = mx.linear_wgrad(dy, ck, bias=bias is not None)
+    return dw.view(weight.shape), db
+
+
+class Conv2dCkptFn(Function):
+    """Conv2dFn (no fused ReLU, no deferred BN) that keeps its input in e4m3 for the weight gradient.  A 1x1 / stride-1 convolution's
+    gradient reads the codes themselves; any other shape writes the values out again for the time of its own backward."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, stride, pad, bn_stats=False):
+        Co, Ci, KH, KW = weight.shape
+        N, H, W, Cx = x.shape
+        assert Cx == rup(Ci, 16), f"conv input has {Cx} channels, weight expects {Ci}"
+        ck = _input_checkpoint(x)
+        y = _igemm(x, pack_weight(weight, 1, x.dtype), bias, None, Co, KH, KW, stride, pad, False, False, conv_out(H, KH, stride, pad),
+                   conv_out(W, KW, stride, pad), bn_stats=bn_stats)
+        ctx.save_for_backward(ck.buffer, weight)
+        ctx.ck_meta = ck.meta
+        ctx.cfg = (stride, pad)
+        ctx.bias_ref = bias
+        ctx.order = SideGrads.next_order()
+        ctx.cell = cell_of(x)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        buffer, weight = ctx.saved_tensors
+        ck = mx.MXTensor.of(buffer, ctx.ck_meta)
+        (stride, pad), bias = ctx.cfg, ctx.bias_ref
+        Co, Ci, KH, KW = weight.shape
+        need = ctx.needs_input_grad
+        dy = dy.contiguous()
+        if (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
+            dw = db = None
+            if need[1]:
+                dw, db = _ckpt_wgrad(dy, ck, weight, bias, ctx.order)
+            dx = _conv2d_bwd(_shape_only(ck), weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order,
+                             (need[0], False, False))[0]
+        else:
+            x = mx.dequantize(ck) if need[1] else _shape_only(ck)
+            dx, dw, db = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, need[:3])
+        return dx, dw, db, None, None, None
+
+
 def _cat_args(xs):
     """(x0..x5, c0..c5, nsrc) of cn_conv1x1_cat_fwd"""
     if len(xs) > 6:
@@ -778,13 +852,16 @@ class Conv1x1CatFn(Function):
     weight fp32 [Co, sum C_s, 1, 1]; every C_s a multiple of 16."""
 
     @staticmethod
-    def forward(ctx, weight, bn_stats, *xs):
+    def forward(ctx, weight, bn_stats, ckpt, *xs):
+        """ckpt: keep the sources in e4m3 (Conv2dCkptFn)"""
         Co = weight.shape[0]
         cells = [cell_of(t) for t in xs]
+        cks = [_input_checkpoint(t) for t in xs] if ckpt else None
         xs = tuple(t.contiguous() for t in xs)
         assert sum(t.shape[-1] for t in xs) == weight.shape[1], "Root conv: channel counts of the children do not add up"
         y = conv1x1_cat_raw(xs, pack_weight(weight, 1, xs[0].dtype), None, None, Co, False, bn_stats=bn_stats)
-        ctx.save_for_backward(weight, *xs)
+        ctx.save_for_backward(weight, *([c.buffer for c in cks] if ckpt else xs))
+        ctx.ck_metas = [c.meta for c in cks] if ckpt else None
         ctx.order = SideGrads.next_order()
         ctx.cells = cells
         return y
@@ -793,8 +870,15 @@ class Conv1x1CatFn(Function):
     def backward(ctx, dy):
         weight, *xs = ctx.saved_tensors
         Co, Ct = weight.shape[:2]
-        N, H, W, _ = xs[0].shape
         dy = dy.contiguous()
+        kept, dy_w = xs, dy                           # what the weight gradient reads, and outlives this call on the side stream
+        cks = None
+        if ctx.ck_metas is not None:
+            cks = [mx.MXTensor.of(b, m) for b, m in zip(xs, ctx.ck_metas)]
+            xs = [_shape_only(c) for c in cks]
+            if dy.shape[-1] != Co:
+                dy_w = dy[..., :Co].contiguous()
+        N, H, W, _ = xs[0].shape
         dt = xs[0].dtype
         chans = [t.shape[-1] for t in xs]
         offs = [sum(chans[:i]) for i in range(len(xs))]
@@ -805,32 +889,32 @@ class Conv1x1CatFn(Function):
                 dw = zeros((Co, Ct), torch.float32, dy.device)
 
             def wgrads(into):
-                for x, c, k0 in zip(xs, chans, offs):
-                    dwp, _ = _wgrad(x, dy, Co, 1, 1, 1, 0, False)               # [rup32(Co)][c]
+                for i, (c, k0) in enumerate(zip(chans, offs)):
+                    dwp = mx.linear_wgrad(dy_w, cks[i])[0] if cks else _wgrad(xs[i], dy, Co, 1, 1, 1, 0, False)[0]      # [>= Co][c]
                     call("cn_unpack_wgrad_cols", dwp, into.view(Co, Ct)[:, k0:], Co, c, c, Ct, int(into is weight.grad))
             if side:
                 def side_work():
                     wgrads(weight.grad)
                     GradReady.note(weight)
-                SideGrads.submit(side_work, dy, *xs, claims=(weight,))
+                SideGrads.submit(side_work, dy_w, *kept, claims=(weight,))
             else:
                 wgrads(dw)
                 dw = dw.view(Co, Ct, 1, 1)
         dxs = [None] * len(xs)
-        if any(ctx.needs_input_grad[2:]):             # inputs: weight, bn_stats flag, *xs
+        if any(ctx.needs_input_grad[3:]):             # inputs: weight, bn_stats and ckpt flags, *xs
             wpd = pack_weight(weight, 0, dt)          # rows = input channel (of the concatenation), k = rup(Co, 16)
             for i, (c, k0) in enumerate(zip(chans, offs)):
-                if ctx.needs_input_grad[2 + i]:
+                if ctx.needs_input_grad[3 + i]:
                     cell = ctx.cells[i]
                     acc = cell.take(like=xs[i]) if cell is not None else None      # shared child: sum in the epilogue
                     dxs[i] = _igemm(dy, wpd[k0:k0 + c], None, acc, c, 1, 1, 1, 0, True, False, H, W)
                     if cell is not None:
                         dxs[i] = cell.give(dxs[i])
-        return (dw, None, *dxs)
+        return (dw, None, None, *dxs)
 
 
-def conv1x1_cat(xs, weight, bn_stats=False):
-    return BnStats.pop(Conv1x1CatFn.apply(weight, bn_stats, *xs)) if bn_stats else Conv1x1CatFn.apply(weight, False, *xs)
+def conv1x1_cat(xs, weight, bn_stats=False, ckpt=False):
+    return BnStats.pop(Conv1x1CatFn.apply(weight, bn_stats, ckpt, *xs)) if bn_stats else Conv1x1CatFn.apply(weight, False, ckpt, *xs)
 
 
 class ConvTranspose2dFn(Function):
@@ -920,6 +1004,29 @@ class StemConvFn(Function):
 
 
 # ------------------------------------------------------------------------------------------------ batch norm
+def _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part):
+    """-> (y, stats [4][C] = mean, invstd, scale, shift) of a training-mode BatchNorm2d + residual + ReLU; part: see BatchNormActFn"""
+    C = x.shape[-1]
+    npix = x.numel() // C
+    y = torch.empty_like(x)
+    stats = torch.empty((4, C), dtype=torch.float32, device=x.device)     # mean, invstd, scale, shift
+    mean, invstd, ss = stats[0], stats[1], stats[2:]
+    ws, n = _bn_ws(npix, C, x.device)
+    if part is not None and BnStats.fused:
+        clear = BnStats.retire(part)          # one launch: the apply kernel reduces the sink, and zeroes the one consumed before it
+        call("cn_bn_train_fwd_sink", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+             part, part.shape[0], clear, clear.numel() if clear is not None else 0, npix, C, BN_MOMENTUM, BN_EPS, int(relu),
+             dtype_code(x.dtype))
+    elif part is not None:
+        call("cn_bn_train_fwd_stats", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+             part, part.shape[0], npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
+        BnStats.release(part)                 # handed back all-zero
+    else:
+        call("cn_bn_train_fwd", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+             npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
+    return y, stats
+
+
 class BatchNormActFn(Function):
     """Training-mode BatchNorm2d + optional residual add + optional ReLU (one fused apply pass)."""
 
@@ -927,24 +1034,7 @@ class BatchNormActFn(Function):
     def forward(ctx, x, gamma, beta, running_mean, running_var, residual, relu, part=None):
         """part: the statistics sink the kernel that produced x filled in its epilogue (BnStats) — x is then read once, by the
         apply pass, instead of twice"""
-        C = x.shape[-1]
-        npix = x.numel() // C
-        y = torch.empty_like(x)
-        stats = torch.empty((4, C), dtype=torch.float32, device=x.device)     # mean, invstd, scale, shift
-        mean, invstd, ss = stats[0], stats[1], stats[2:]
-        ws, n = _bn_ws(npix, C, x.device)
-        if part is not None and BnStats.fused:
-            clear = BnStats.retire(part)          # one launch: the apply kernel reduces the sink, and zeroes the one consumed before it
-            call("cn_bn_train_fwd_sink", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-                 part, part.shape[0], clear, clear.numel() if clear is not None else 0, npix, C, BN_MOMENTUM, BN_EPS, int(relu),
-                 dtype_code(x.dtype))
-        elif part is not None:
-            call("cn_bn_train_fwd_stats", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-                 part, part.shape[0], npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
-            BnStats.release(part)                 # handed back all-zero
-        else:
-            call("cn_bn_train_fwd", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-                 npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
+        y, stats = _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part)
         # ReLU backward mask: without a residual input it is recomputed from x and the saved affine (y is not re-read)
         need_y = relu and residual is not None
         ctx.save_for_backward(x, y if need_y else None, gamma, stats)
@@ -999,6 +1089,41 @@ class BatchNormActFn(Function):
         dgamma = torch.empty(C, dtype=torch.float32, device=x.device)
         dbeta = torch.empty(C, dtype=torch.float32, device=x.device)
         run(dgamma, dbeta, 0)
+        return dx, dgamma, dbeta, None, None, (cell.give(dres) if cell is not None else dres), None, None
+
+
+class BatchNormCkptFn(Function):
+    """BatchNormActFn with an 8-bit backward: what is kept of the input is its e4m3 checkpoint (and, behind a ReLU, one sign bit of each
+    output), 8.25 - 9.25 bits a value instead of 16 / 32 — and the output need not be kept for the mask either.  The forward result is
+    BatchNormActFn's, bit for bit."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, running_mean, running_var, residual, relu, part=None):
+        y, stats = _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part)
+        ck = mx.checkpoint(x, sign_of=y if relu else None)
+        ctx.save_for_backward(ck.buffer, gamma, stats)
+        ctx.ck_meta = ck.meta
+        ctx.beta_ref = beta
+        ctx.has_res = residual is not None
+        ctx.res_cell = cell_of(residual)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        buffer, gamma, stats = ctx.saved_tensors
+        ck = mx.MXTensor.of(buffer, ctx.ck_meta)
+        filled = BnBwdSinks.take(dy)               # sums a producer of dy may have left are over the unquantised input: not these
+        if filled is not None:
+            filled.zero_()
+            BnStats.release(filled)
+        beta, cell = ctx.beta_ref, ctx.res_cell if ctx.has_res else None
+        racc = cell.take(like=dy) if cell is not None else None
+        side = SideGrads.usable(gamma, beta)
+        dx, dgamma, dbeta, dres = mx.batch_norm_act_bwd(dy, ck, gamma.detach(), stats[0], stats[1], residual=ctx.has_res, racc=racc,
+                                                        into=(gamma.grad, beta.grad) if side else None)
+        if side:
+            GradReady.note(gamma, beta)
+            dgamma = dbeta = None
         return dx, dgamma, dbeta, None, None, (cell.give(dres) if cell is not None else dres), None, None
 
 
@@ -1887,12 +2012,19 @@ def conv2d(x, weight, bias=None, stride=1, pad=0, relu=False, mask_dx=False, def
     return out
 
 
+def conv2d_ckpt(x, weight, bias=None, stride=1, pad=0, bn_stats=False):
+    """conv2d whose input is kept in e4m3 for its weight gradient (mx.checkpoint)"""
+    y = Conv2dCkptFn.apply(x, weight, bias, stride, pad, bn_stats)
+    return BnStats.pop(y) if bn_stats else y
+
+
 def conv_transpose2d(x, weight, stride=2, pad=1):
     return ConvTranspose2dFn.apply(x, weight, stride, pad)
 
 
-def batch_norm_act(x, bn, residual=None, relu=True):
-    return BatchNormActFn.apply(x, bn.weight, bn.bias, bn.running_mean, bn.running_var, residual, relu, getattr(x, "_bn_part", None))
+def batch_norm_act(x, bn, residual=None, relu=True, ckpt=False):
+    """ckpt: keep the input in e4m3 and the ReLU's mask in bits for the backward pass"""
+    return (BatchNormCkptFn if ckpt else BatchNormActFn).apply(x, bn.weight, bn.bias, bn.running_mean, bn.running_var, residual, relu, getattr(x, "_bn_part", None))
 
 
 def max_pool(x, k, stride, pad=0):
