@@ -35,9 +35,10 @@ template <typename T> struct MxBnRow {
         q = reinterpret_cast<const uint2*>(g.codes)[i];
         b = g.scales[r * g.blocks + (c >> 2)];
         m = SIGNS ? g.signs[i] : 0u;
-        dy.template load<FULL>(reinterpret_cast<const T*>(g.dy), r * g.C + c * 8, left, true);
+        dy.template load<FULL>(reinterpret_cast<const T*>(g.dy), r * g.C + c * 8, left, true, g.C);
     }
-    template <bool SIGNS> __device__ inline void get(float (&d)[8], float (&v)[8]) const {
+    template <bool SIGNS, bool FULL> __device__ inline void get(float (&d)[8], float (&v)[8]) {
+        dy.template fix<FULL>();
         dy.get(d);
         if (SIGNS) {
 #pragma unroll
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
             for (int u = 0; u < MXBN_U; ++u) {
                 if (r + u * nrl < r1) {
                     float d[8], v[8];
-                    row[u].template get<SIGNS>(d, v);
+                    row[u].template get<SIGNS, FULL>(d, v);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
                 }
@@ -154,7 +155,8 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
     float ka[8], kb[8], kc[8], mu[8];
     auto get = [&](const float* p, float (&o)[8]) {
         MxRaw8<float> k;
-        k.template load<FULL>(p, c * 8, left, true);
+        k.template load<FULL>(p, c * 8, left, true, g.C);
+        k.template fix<FULL>();
         k.get(o);
     };
     get(mean, mu);
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
         for (int u = 0; u < MXBN_U; ++u) {
             if (r + u * nrl < r1) {
                 float d[8], v[8], o[8];
-                row[u].template get<SIGNS>(d, v);
+                row[u].template get<SIGNS, FULL>(d, v);
                 const int64_t at = (r + u * nrl) * g.C + c * 8;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = fmaf(ka[j], d[j], -fmaf(kb[j], v[j] - mu[j], kc[j]));

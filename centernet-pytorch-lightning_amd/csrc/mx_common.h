@@ -83,23 +83,40 @@ __device__ static inline void mx_store8(bf16_t* p, int left, const float (&v)[8]
     }
 }
 
-// Eight consecutive elements as they lie in memory, so that several loads can be in flight before the first is unpacked.  FULL: the row
-// has a multiple of 8 channels, so a chunk lies inside it or outside (branch-free: a readable address, masked; an exec-masked branch
-// would make the compiler wait for every load before the next); otherwise the row's last chunk is read element by element.
+// Eight consecutive elements as they lie in memory, so that several loads can be in flight before the first is unpacked (an exec-masked
+// branch would make the compiler wait for every load before the next: these have none).  `left`: channels of the row from here on (may
+// be <= 0), `ok`: the row exists; what is not there reads as zero.  FULL: the row has a multiple of 8 channels, so a chunk lies inside
+// it or outside.  Otherwise the row's last chunk is read eight elements before the row's end and shifted down; rows of fewer than eight
+// channels (C < 8, the same for all lanes) are read element by element.
+// A load leaves raw bits and what is wrong with them (s: elements to shift down, 8: nothing was there); `fix` puts that right, at the time
+// of use — done at once it would make every load wait for the one before.
+__device__ static inline u32x4_t mx_pick(bool c, u32x4_t a, u32x4_t b) { return u32x4_t{c ? a.x : b.x, c ? a.y : b.y, c ? a.z : b.z, c ? a.w : b.w}; }
 template <typename T> struct MxRaw8;
 template <> struct MxRaw8<bf16_t> {
     u32x4_t a;
-    template <bool FULL> __device__ inline void load(const bf16_t* base, int64_t at, int left, bool ok) {
-        if (FULL) {
-            ok = ok && left > 0;
-            const u32x4_t v = *reinterpret_cast<const u32x4_a2*>(base + (ok ? at : 0));
-            const uint32_t m = ok ? 0xffffffffu : 0u;
-            a = u32x4_t{v.x & m, v.y & m, v.z & m, v.w & m};
-        } else {
-            float f[8];
-            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
-            a = u32x4_t{pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7])};
+    int s;
+    template <bool FULL> __device__ inline void load(const bf16_t* base, int64_t at, int left, bool ok, int C) {
+        ok = ok && left > 0;
+        if (!FULL && C < 8) {
+            uint32_t e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = ok && i < left ? base[at + i] : 0u;
+            a = u32x4_t{e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16};
+            s = 0;
+            return;
         }
+        s = !ok ? 8 : (FULL || left >= 8 ? 0 : 8 - left);
+        a = *reinterpret_cast<const u32x4_a2*>(base + (ok ? at - s : 0));
+    }
+    template <bool FULL> __device__ inline void fix() {
+        const uint32_t m = s & 8 ? 0u : 0xffffffffu;
+        if (!FULL) {
+            u32x4_t v = mx_pick(s & 4, u32x4_t{a.z, a.w, 0u, 0u}, a);
+            v = mx_pick(s & 2, u32x4_t{v.y, v.z, v.w, 0u}, v);
+            const uint32_t h = (s & 1) * 16;
+            a = u32x4_t{__builtin_amdgcn_alignbit(v.y, v.x, h), __builtin_amdgcn_alignbit(v.z, v.y, h), __builtin_amdgcn_alignbit(v.w, v.z, h), v.w >> h};
+        }
+        a = u32x4_t{a.x & m, a.y & m, a.z & m, a.w & m};
     }
     __device__ inline void get(float (&f)[8]) const {
 #pragma unroll
@@ -108,27 +125,44 @@ template <> struct MxRaw8<bf16_t> {
 };
 template <> struct MxRaw8<float> {
     u32x4_t a, b;
-    template <bool FULL> __device__ inline void load(const float* base, int64_t at, int left, bool ok) {
-        if (FULL) {
-            ok = ok && left > 0;
-            const float* p = base + (ok ? at : 0);
-            const u32x4_t v = *reinterpret_cast<const u32x4_a4*>(p), w = *reinterpret_cast<const u32x4_a4*>(p + 4);
-            const uint32_t m = ok ? 0xffffffffu : 0u;
-            a = u32x4_t{v.x & m, v.y & m, v.z & m, v.w & m};
-            b = u32x4_t{w.x & m, w.y & m, w.z & m, w.w & m};
-        } else {
-            float f[8];
-            mx_load8(base + (ok ? at : 0), ok ? left : 0, f);
+    int s;
+    template <bool FULL> __device__ inline void load(const float* base, int64_t at, int left, bool ok, int C) {
+        ok = ok && left > 0;
+        if (!FULL && C < 8) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i] = __float_as_uint(f[i]); b[i] = __float_as_uint(f[4 + i]); }
+            for (int i = 0; i < 4; ++i) {
+                a[i] = ok && i < left ? __float_as_uint(base[at + i]) : 0u;
+                b[i] = ok && i + 4 < left ? __float_as_uint(base[at + i + 4]) : 0u;
+            }
+            s = 0;
+            return;
         }
+        s = !ok ? 8 : (FULL || left >= 8 ? 0 : 8 - left);
+        const float* p = base + (ok ? at - s : 0);
+        a = *reinterpret_cast<const u32x4_a4*>(p);
+        b = *reinterpret_cast<const u32x4_a4*>(p + 4);
+    }
+    template <bool FULL> __device__ inline void fix() {
+        const u32x4_t z = {0u, 0u, 0u, 0u};
+        if (!FULL) {
+            a = mx_pick(s & 4, b, a);
+            b = mx_pick(s & 4, z, b);
+            const u32x4_t a2 = {a.z, a.w, b.x, b.y}, b2 = {b.z, b.w, 0u, 0u};
+            a = mx_pick(s & 2, a2, a);
+            b = mx_pick(s & 2, b2, b);
+            const u32x4_t a1 = {a.y, a.z, a.w, b.x}, b1 = {b.y, b.z, b.w, 0u};
+            a = mx_pick(s & 1, a1, a);
+            b = mx_pick(s & 1, b1, b);
+        }
+        const uint32_t m = s & 8 ? 0u : 0xffffffffu;
+        a = u32x4_t{a.x & m, a.y & m, a.z & m, a.w & m};
+        b = u32x4_t{b.x & m, b.y & m, b.z & m, b.w & m};
     }
     __device__ inline void get(float (&f)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(a[i]); f[4 + i] = __uint_as_float(b[i]); }
     }
 };
-
 // store of eight elements of such a row (FULL as above)
 template <bool FULL, typename T> __device__ static inline void mx_store8f(T* p, int left, const float (&v)[8]) {
     if (FULL) { if (left > 0) mx_store8(p, 8, v); }

@@ -81,7 +81,7 @@ template <int NJ> struct MxLinB { u32x4_t f[2][NJ]; };
 
 // MI x NJ tiles of 32 x 32 per wave; WM x WN waves over rows and columns, WK over the channels (few rows: the launch would be short of
 // waves otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows
-template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULL, bool resident>
+template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN, bool resident>
 __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
     static_assert(WM * WN * WK == 4 && (WK == 1 || (WK == 4 && MI == 1)), "four waves");
     constexpr int BM = 32 * MI * WM, EPN = 32 * NJ, EPP = EPN + 4;         // EPP: floats per staged output row (rows on different banks)
@@ -105,11 +105,12 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
                 row[u] = (int)mx_quot(i, dv);
                 pc[u] = (int)i - row[u] * (int)dv.d;
                 const int c0 = s0 * 64 + pc[u] * 8;
-                v[u].template load<FULL>(X, (int64_t)row[u] * g.K + c0, g.K - c0, (int)i < total);
+                v[u].template load<FULLK>(X, (int64_t)row[u] * g.K + c0, g.K - c0, (int)i < total, g.K);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[8];
+                v[u].template fix<FULLK>();
                 v[u].get(f);
                 const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(mx_absmax8(f)));
                 if (base + u * 256 < total) {                     // (whole quads)
@@ -156,12 +157,13 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
         }                                                                                                                               \
     }
     // eight finished columns of a row; rv: the residual input there (zeros: none)
-    auto finish = [&](float (&v)[8], const MxRaw8<T>& rv, int64_t m, int nc, int left, const float (&bs)[8]) {
-        float r[8];
-        rv.get(r);
+    auto finish = [&](float (&v)[8], MxRaw8<T>& rv, int64_t m, int nc, int left, const float (&bs)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bs[e];
         if (g.res) {
+            float r[8];
+            rv.template fix<FULLN>();
+            rv.get(r);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] += r[e];
         }
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];            // (a NaN stays one)
         }
-        if (m < g.M) mx_store8f<FULL>(reinterpret_cast<T*>(g.y) + m * g.N + nc, left, v);
+        if (m < g.M) mx_store8f<FULLN>(reinterpret_cast<T*>(g.y) + m * g.N + nc, left, v);
     };
 
     MxLinB<NJ> B0, B1;
@@ -191,7 +193,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 #pragma unroll
             for (int q = 0; q < MI * 2 * NQ; ++q) {
                 const int64_t m = m0 + wm * MI * 32 + q * RPI + lane / LPR;
-                rv[q].template load<FULL>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M);
+                rv[q].template load<FULLN>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M, g.N);
             }
         }
 #pragma unroll
@@ -234,7 +236,8 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
         for (int e = 0; e < 8; ++e) bs[e] = 0.f;
         if (g.bias) {
             MxRaw8<float> b;
-            b.template load<FULL>(g.bias, nc, left, true);
+            b.template load<FULLN>(g.bias, nc, left, true, g.N);
+            b.template fix<FULLN>();
             b.get(bs);
         }
         if (WK == 1) {
@@ -267,7 +270,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
                 for (int e = 0; e < 16; ++e) ep[(wk * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[0][j][e];
             __syncthreads();
             for (int r = tid / LPR; r < rows; r += 256 / LPR) {
-                if (g.res) rv[0].template load<FULL>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true);
+                if (g.res) rv[0].template load<FULLN>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true, g.N);
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = 0.f;
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 #undef MXL_STEP
 }
 
-template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULL>
+template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN>
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
     constexpr int BM = 32 * MI * WM, EPP = 32 * NJ + 4;
     const int ep = (WK > 1 ? 4 * 32 : 4 * 16) * EPP * 4;
@@ -315,23 +318,23 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     int dev = 0;
     CN_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (dev < 64) attr[dev] = true;
     }
     const dim3 grid((unsigned)mt, (unsigned)split);
-    if (chunk >= g.S) mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, true><<<grid, 256, smem, st>>>(g);
-    else mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULL, false><<<grid, 256, smem, st>>>(g);
+    if (chunk >= g.S) mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, 256, smem, st>>>(g);
+    else mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, 256, smem, st>>>(g);
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
 }
-template <typename T, bool FULL>
+template <typename T, bool FULLK, bool FULLN>
 static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
     // few rows: less than one 64 x 256 workgroup for each compute unit
-    if ((g.M + 63) / 64 * cdiv(g.N, 256) < 256) return mxl_launch<T, 1, 1, 1, 1, 4, FULL>(g, st);
-    if (g.N <= 64) return mxl_launch<T, 1, 2, 4, 1, 1, FULL>(g, st);
-    if (g.N <= 128) return mxl_launch<T, 1, 2, 2, 2, 1, FULL>(g, st);
-    return mxl_launch<T, 1, 2, 1, 4, 1, FULL>(g, st);
+    if ((g.M + 63) / 64 * cdiv(g.N, 256) < 256) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
+    if (g.N <= 64) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
+    if (g.N <= 128) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
+    return mxl_launch<T, 1, 2, 1, 4, 1, FULLK, FULLN>(g, st);
 }
 
 extern "C" int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const void* residual, void* y, int64_t M, int K, int N,
@@ -356,6 +359,9 @@ extern "C" int cn_mx_linear_fwd(const void* x, const void* packed, const float* 
     g.S4 = cdiv(g.S, 4);
     g.relu = relu;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == CN_BF16) return (K | N) % 8 == 0 ? mxl_choose<bf16_t, true>(g, st) : mxl_choose<bf16_t, false>(g, st);
-    return (K | N) % 8 == 0 ? mxl_choose<float, true>(g, st) : mxl_choose<float, false>(g, st);
+#define MXL_GO(T) do { if (K % 8 == 0) return N % 8 == 0 ? mxl_choose<T, true, true>(g, st) : mxl_choose<T, true, false>(g, st);       \
+                       return N % 8 == 0 ? mxl_choose<T, false, true>(g, st) : mxl_choose<T, false, false>(g, st); } while (0)
+    if (dtype == CN_BF16) MXL_GO(bf16_t);
+    MXL_GO(float);
+#undef MXL_GO
 }

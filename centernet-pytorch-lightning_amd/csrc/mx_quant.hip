@@ -19,14 +19,15 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
         const uint32_t l = threadIdx.x + u * 256, n = rem0 + l, r = mx_quot(n, cpr);
         const int c0 = (int)(n - r * cpr.d) * 8;
         const int64_t at = (row0 + r) * C + c0;
-        v[u].template load<FULL>(x, at, C - c0, base + l < chunks);
-        if (SIGNS) w[u].template load<FULL>(sg, at, C - c0, base + l < chunks);
+        v[u].template load<FULL>(x, at, C - c0, base + l < chunks, C);
+        if (SIGNS) w[u].template load<FULL>(sg, at, C - c0, base + l < chunks, C);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t i = base + threadIdx.x + u * 256;
         if (i >= chunks) return;                                         // (chunks is a multiple of 4: a quad stays whole)
         float f[8];
+        v[u].template fix<FULL>();
         v[u].get(f);
         const uint32_t b = mx_scale_byte<FMT>(quad_max_u(mx_absmax8(f)));
         if (FMT == CN_MX_E2M1) reinterpret_cast<uint32_t*>(codes)[i] = mx_codes_e2m1(f, b);
@@ -34,6 +35,7 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
         if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)b;
         if (SIGNS) {
             float s[8];
+            w[u].template fix<FULL>();
             w[u].get(s);
             uint32_t m = 0;
 #pragma unroll

@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
 #pragma unroll
             for (int v = 0; v < YV; ++v) {
                 const int r = yr + v * (256 / YC);
-                w.y[v].template load<false>(reinterpret_cast<const T*>(g.dy), (rr + r) * g.N + n0 + yc, yleft, r < left);
+                w.y[v].template load<false>(reinterpret_cast<const T*>(g.dy), (rr + r) * g.N + n0 + yc, yleft, r < left, g.N);
             }
         }
         const auto bx = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(g.codes + rr * g.Kp), 0, (uint32_t)left * g.Kp, 0x00020000);
@@ -127,9 +127,10 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     float sb[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sb[j] = 0.f;
-    auto lstore = [&](const Raw& w) {
+    auto lstore = [&](Raw& w) {
 #pragma unroll
         for (int v = 0; v < YV; ++v) {
+            if (!FULL) w.y[v].template fix<false>();              // (ranged buffer loads leave nothing to put right)
             mx_put_dy(w.y[v], ly + (yr + v * (256 / YC)) * YP + yc, PLANE);
             if (bias) {
                 float f[8];
