@@ -216,6 +216,88 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
     }
 }
 
+// Few rows: everything in one launch.  A thread keeps its U rows of a chunk in registers between the sums and dx, so a workgroup (all
+// rows of 2^lg chunks) reads its inputs once.  The chunks of a cache line belong to neighbouring workgroups: these are dealt to one XCD.
+template <typename T, bool SIGNS, bool FULL, int U>
+__global__ __launch_bounds__(256) void mx_bn_small_kernel(const MxBnGeom g, const float* __restrict__ mean, const MxBnTail t,
+                                                          T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc, int wgs) {
+    __shared__ float red[4][4 * 16];
+    const int per = (wgs + 7) / 8, wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || wg >= wgs) return;       // (the grid is 8 x per)
+    const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
+    const int c = wg * tc + cl, left = g.C - c * 8;
+    MxBnRow<T> row[U];
+    float mu[8], s0[8], s1[8];
+    auto get = [&](const float* p, float (&o)[8]) {
+        MxRaw8<float> k;
+        k.template load<FULL>(p, c * 8, left, true, g.C);
+        k.template fix<FULL>();
+        k.get(o);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) row[u].template load<SIGNS, FULL>(g, rl + u * nrl, left > 0 ? c : 0, left, left > 0 && rl + u * nrl < g.rows);
+    get(mean, mu);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (rl + u * nrl < g.rows) {
+            float d[8], v[8];
+            row[u].template get<SIGNS, FULL>(d, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
+        }
+    }
+    for (int o = 32; o >= tc; o >>= 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { s0[j] += __shfl_xor(s0[j], o, 64); s1[j] += __shfl_xor(s1[j], o, 64); }
+    }
+    if ((tid & 63) < tc) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { red[tid >> 6][cl * 16 + j] = s0[j]; red[tid >> 6][cl * 16 + 8 + j] = s1[j]; }
+    }
+    __syncthreads();
+    if (left <= 0) return;
+    float is[8], ga[8], ka[8], kb[8], kc[8];
+    get(t.invstd, is);
+    get(t.gamma, ga);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int a = cl * 16 + j, b = a + 8;
+        const float t0 = (red[0][a] + red[1][a]) + (red[2][a] + red[3][a]), t1 = (red[0][b] + red[1][b]) + (red[2][b] + red[3][b]);
+        const float dg = t1 * is[j];
+        ka[j] = ga[j] * is[j];
+        kb[j] = ka[j] * is[j] * dg * t.inv_rows;
+        kc[j] = ka[j] * t0 * t.inv_rows;
+        if (rl == 0 && j < left) {
+            t.dgamma[c * 8 + j] = t.accumulate ? t.dgamma[c * 8 + j] + dg : dg;
+            t.dbeta[c * 8 + j] = t.accumulate ? t.dbeta[c * 8 + j] + t0 : t0;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t r = rl + u * nrl;
+        if (r < g.rows) {
+            float d[8], v[8], o[8];
+            row[u].template get<SIGNS, true>(d, v);               // (put right above)
+            const int64_t at = r * g.C + c * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(ka[j], d[j], -fmaf(kb[j], v[j] - mu[j], kc[j]));
+            mx_store8f<FULL>(dx + at, left, o);
+            if (dres) {
+                if (racc) {
+                    mx_load8(racc + at, left, o);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) d[j] += o[j];
+                }
+                mx_store8f<FULL>(dres + at, left, d);
+            }
+        }
+    }
+}
+
+#define MXBN_SMALL 2048        // rows that 256 threads hold eight of each
+
 static int mxbn_lg(int C) {
     const int chunks = cdiv(C, 8);
     int lg = 0;
@@ -233,7 +315,7 @@ static int mxbn_groups(int64_t rows, int C) {
 }
 
 extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C) {
-    if (rows < 1 || C < 1 || C > MX_MAX_C) return 0;
+    if (rows <= MXBN_SMALL || C < 1 || C > MX_MAX_C) return 0;
     return sizeof(float) * ((size_t)mxbn_groups(rows, C) * 2 + 3) * (size_t)C;
 }
 
@@ -245,11 +327,29 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     CN_CHECK_ARG(dy && codes && scales && gamma && mean && invstd && dx && dgamma && dbeta, "cn_mx_bn_bwd: null pointer");
     CN_CHECK_ARG(dres || !racc, "cn_mx_bn_bwd: racc without dres");
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_bn_bwd: codes must be 16-byte aligned");
-    if (!ws || ws_bytes < cn_mx_bn_bwd_bytes(rows, C)) {
+    if (ws_bytes < cn_mx_bn_bwd_bytes(rows, C) || (!ws && ws_bytes)) {
         cn_set_error("cn_mx_bn_bwd: workspace of %zu bytes needed", cn_mx_bn_bwd_bytes(rows, C));
         return CN_EWORKSPACE;
     }
     hipStream_t st = (hipStream_t)stream;
+    const bool full = C % 8 == 0;
+#define MXBN_GO(KERNEL, MORE, GRID, ...)                                                                                               \
+    CN_DISPATCH_DTYPE(dtype, T, {                                                                                                      \
+        if (signs) { if (full) KERNEL<T, true, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, true, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }  \
+        else { if (full) KERNEL<T, false, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, false, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }      \
+    })
+#define MXBN_COMMA ,
+    if (rows <= MXBN_SMALL) {
+        MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 0};
+        const MxBnTail t{nullptr, nullptr, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, 0, accumulate};
+        // four, two or one chunk a workgroup: eight rows a thread at most (two where that is enough)
+        g.lg = rows <= 512 ? 2 : (rows <= 1024 ? 1 : 0);
+        const int wgs = cdiv(cdiv(C, 8), 1 << g.lg), grid = cdiv(wgs, 8) * 8;
+        if (rows <= 2 * (256 >> g.lg)) MXBN_GO(mx_bn_small_kernel, MXBN_COMMA 2, grid, g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs);
+        else MXBN_GO(mx_bn_small_kernel, MXBN_COMMA 8, grid, g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs);
+        CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+        return CN_OK;
+    }
     const int groups = mxbn_groups(rows, C);
     float* part = (float*)ws;
     float* coef = part + (size_t)groups * 2 * C;
@@ -258,13 +358,6 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     const int nrl = 256 >> g.lg;
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
     g.per = (rows + groups - 1) / groups;
-    const bool full = C % 8 == 0;
-#define MXBN_GO(KERNEL, MORE, GRID, ...)                                                                                               \
-    CN_DISPATCH_DTYPE(dtype, T, {                                                                                                      \
-        if (signs) { if (full) KERNEL<T, true, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, true, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }  \
-        else { if (full) KERNEL<T, false, true MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); else KERNEL<T, false, false MORE><<<GRID, 256, 0, st>>>(__VA_ARGS__); }      \
-    })
-#define MXBN_COMMA ,
     MXBN_GO(mx_bn_sums_kernel, , dim3(groups, tiles), g, mean, part);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     const MxBnTail t{coef, part, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, groups, accumulate};

@@ -265,22 +265,24 @@ __global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* __restr
 }
 
 // Tiles and splits.  Large problems take the wide tiles (a row of dy / x8 is read again for every K / N tile) and two workgroups a compute
-// unit; small ones the narrow tiles, whose workgroups are short of work sooner, and no split once the tiles alone fill the card (each
-// split writes and reads a whole dw).  us, wide | narrow, bf16: 262144x256x128 43 | 66, 65536x1024x256 54 | 93, 16384x512x2048 55 | 96;
-// 8192x512x512 24.2 | 21.5, 65536x256x64 18.3 | 15.2, 4096x1024x256 18.9 | 15.9, 1024x2048x512 14.0 | 11.8 (15.1 in two splits).
-// 32 bits (64 x 128 | 64 x 64): 65536x1024x256 139 | 199, 65536x256x64 19.8 | 21.5, 30000x80x208 20.2 | 23.5; 512x256x256 9.0 | 8.1.
+// unit; small ones the narrow tiles, whose workgroups are short of work sooner.  A split writes and reads a whole dw and the join is a
+// launch of its own: none once the tiles alone fill the card, or for a few rows of many tiles, and two row tiles to a split at least.
+// us, wide | narrow, bf16: 262144x256x128 43 | 56, 65536x1024x256 53 | 72, 16384x512x2048 56 | 74, 25394x224x660 31 | 46;
+// 8192x512x512 24.3 | 21.8, 65536x256x64 18.5 | 15.2, 4096x1024x256 19.1 | 16.5, 1024x2048x512 18.3 | 12.4 (15.8 in two splits),
+// 204x800x732 7.4 (10.6 in two splits), 15993x22x51 10.9 (13.2 with a row tile a split).
+// 32 bits (64 x 128 | 64 x 64): 65536x1024x256 137 | 176, 65536x256x64 20.4 | 22.7, 30000x80x208 20.2 | 24.0; 831x864x560 17.1 | 16.2.
 struct MxWgPlan { bool wide; int tn, tk, ntiles, ktiles, splits; int64_t per; };
 static MxWgPlan mxwg_plan(int64_t rows, int K, int N, int dtype) {
     MxWgPlan p;
     const double macs = (double)rows * K * N;
-    p.wide = dtype == CN_BF16 ? (macs >= 4e9 && N > 64 && K > 64) : (macs >= 4e8 && K > 64);
+    p.wide = dtype == CN_BF16 ? (macs >= 3e9 && N > 64 && K > 64) : (macs >= 5e8 && K > 64);
     p.tn = p.wide && dtype == CN_BF16 ? 128 : 64;
     p.tk = p.wide ? 128 : 64;
     p.ntiles = cdiv(N, p.tn);
     p.ktiles = cdiv(K, p.tk);
     const int64_t tiles = (int64_t)p.ntiles * p.ktiles, rtiles = (rows + 63) / 64;
-    int64_t s = tiles >= 192 ? 1 : 512 / tiles;
-    s = s < rtiles ? s : rtiles;
+    int64_t s = tiles >= 192 || (rtiles <= 16 && tiles >= 32) ? 1 : 512 / tiles;
+    s = s < rtiles / 2 ? s : rtiles / 2;
     s = s < 1 ? 1 : s;
     p.per = (rtiles + s - 1) / s * 64;
     p.splits = (int)((rows + p.per - 1) / p.per);
@@ -290,7 +292,7 @@ static MxWgPlan mxwg_plan(int64_t rows, int K, int N, int dtype) {
 extern "C" size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype) {
     if (rows < 1 || K < 1 || N < 1 || K > MX_MAX_C || N > MX_MAX_C) return 0;
     const MxWgPlan p = mxwg_plan(rows, K, N, dtype);
-    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * ((size_t)N * K + N) : 16;
+    return p.splits > 1 ? sizeof(float) * (size_t)p.splits * ((size_t)N * K + N) : 0;
 }
 
 template <typename T, int TN, int TK>
@@ -307,7 +309,7 @@ extern "C" int cn_mx_linear_wgrad(const void* dy, const void* codes, const void*
     CN_CHECK_ARG(dtype == CN_F32 || dtype == CN_BF16, "cn_mx_linear_wgrad: bad dtype %d", dtype);
     CN_CHECK_ARG(dy && codes && scales && dw, "cn_mx_linear_wgrad: null pointer");
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_linear_wgrad: codes must be 16-byte aligned");
-    if (!ws || ws_bytes < cn_mx_linear_wgrad_bytes(rows, K, N, dtype)) {
+    if (ws_bytes < cn_mx_linear_wgrad_bytes(rows, K, N, dtype) || (!ws && ws_bytes)) {
         cn_set_error("cn_mx_linear_wgrad: workspace of %zu bytes needed", cn_mx_linear_wgrad_bytes(rows, K, N, dtype));
         return CN_EWORKSPACE;
     }

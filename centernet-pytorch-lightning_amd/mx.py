@@ -189,7 +189,7 @@ def linear(x, weight, bias=None, residual=None, relu=False):
     x's type.  Serving only: an input that wants a gradient is refused (train in bf16, pack the result)."""
     if not isinstance(weight, MXWeight):
         raise TypeError("mx.linear: weight must come from mx.pack_weight")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, bias, residual)):
+    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(bias, "requires_grad", False) or getattr(residual, "requires_grad", False)):
         raise RuntimeError("mx.linear has no backward pass: call it under torch.no_grad()")
     x, dt = _tensor(x, "mx.linear")
     N, K, dev = weight.out_features, weight.in_features, x.device
@@ -238,10 +238,10 @@ def linear_wgrad(dy, ck, bias=False, into=None, bias_into=None):
                 db.zero_()
         return dw, db
     n = _hip.query("cn_mx_linear_wgrad_bytes", rows, K, N, dt)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     codes, scales, _ = ck._pointers()
     launch("cn_mx_linear_wgrad", dy.get_device(), dy.data_ptr(), codes, scales, dw.data_ptr(), _ptr(db), 0 if into is None else 1, rows, K, N,
-           dt, ws.data_ptr(), n)
+           dt, _ptr(ws), n)
     return dw, db
 
 
@@ -273,8 +273,8 @@ def batch_norm_act_bwd(dy, ck, gamma, mean, invstd, residual=False, racc=None, i
     dx = torch.empty_like(dy)
     dres = torch.empty_like(dy) if residual else None
     n = _hip.query("cn_mx_bn_bwd_bytes", rows, C)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     codes, scales, signs = ck._pointers()
     launch("cn_mx_bn_bwd", dy.get_device(), dy.data_ptr(), codes, scales, signs, gamma.data_ptr(), mean.data_ptr(), invstd.data_ptr(),
-           dx.data_ptr(), _ptr(dres), _ptr(racc), dgamma.data_ptr(), dbeta.data_ptr(), 0 if into is None else 1, rows, C, dt, ws.data_ptr(), n)
+           dx.data_ptr(), _ptr(dres), _ptr(racc), dgamma.data_ptr(), dbeta.data_ptr(), 0 if into is None else 1, rows, C, dt, _ptr(ws), n)
     return dx, dgamma, dbeta, dres

@@ -181,7 +181,7 @@ def test_checkpoint_signs(dt, rows, C):
 
 # ------------------------------------------------------------------------------------------------ product
 LINEAR = [(1, 1, 1), (1, 32, 32), (1, 2048, 512), (2, 64, 80), (31, 16, 64), (33, 77, 5), (64, 100, 200), (65, 513, 130), (129, 208, 65),
-          (200, 1100, 300), (130, 4096, 260), (67, 4500, 70), (300, 2100, 100), (5, 9000, 40), (128, 512, 1024), (1000, 64, 64), (257, 256, 2048)]
+          (200, 1100, 300), (130, 4096, 260), (67, 4500, 70), (300, 2100, 100), (5, 9000, 40), (128, 512, 1024), (1000, 64, 64), (257, 256, 2048), (20000, 72, 4), (40, 2056, 3)]
 
 
 @pytest.mark.parametrize("dt", [BF, F32])
@@ -242,7 +242,7 @@ def test_linear_refusals():
 
 # ------------------------------------------------------------------------------------------------ weight gradient
 WGRAD = [(1, 1, 1), (1, 32, 8), (3, 16, 7), (63, 64, 64), (65, 77, 65), (64, 33, 130), (1000, 80, 208), (5000, 64, 16), (700, 515, 129),
-         (40000, 16, 24), (128, 2048, 130)]
+         (40000, 16, 24), (128, 2048, 130), (200, 808, 732), (4000, 7, 3), (17000, 424, 420)]
 
 
 @pytest.mark.parametrize("dt", [BF, F32])
@@ -301,7 +301,8 @@ def test_linear_wgrad_refusals():
 
 
 # ------------------------------------------------------------------------------------------------ batch norm
-NORM = [(2, 1), (3, 8), (5, 33), (64, 80), (300, 64), (129, 515), (2000, 256), (7, 2048), (30000, 16), (11, 4100)]
+NORM = [(2, 1), (3, 8), (5, 33), (64, 80), (300, 64), (129, 515), (2000, 256), (7, 2048), (30000, 16), (11, 4100), (512, 100), (1024, 24), (2048, 72),
+        (2049, 72), (2100, 13), (9000, 520), (70000, 7)]
 
 
 @pytest.mark.parametrize("dt", [BF, F32])
