@@ -18,6 +18,7 @@ struct MxBnGeom {
     const uint8_t* signs;      // nullptr: no ReLU
     int64_t rows;
     int C, cpr, blocks;        // cpr: 8-channel chunks per (padded) row of codes, blocks = cpr / 4
+    int ld;                    // C rounded up to 8: channels per row of the partial sums and of the coefficients
     int lg;                    // log2 of the chunks a workgroup covers
     int64_t per;               // rows per workgroup
 };
@@ -87,32 +88,25 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
     for (int t = tid; t < tc * 16; t += 256) {
         const float s = (red[t] + red[tc * 16 + t]) + (red[2 * tc * 16 + t] + red[3 * tc * 16 + t]);
         const int ch = (blockIdx.y * tc + (t >> 4)) * 8 + (t & 7);
-        if (ch < g.C) part[((int64_t)blockIdx.x * 2 + ((t >> 3) & 1)) * g.C + ch] = s;
+        if (ch < g.ld) part[((int64_t)blockIdx.x * 2 + ((t >> 3) & 1)) * g.ld + ch] = s;      // (zeros behind the last channel)
     }
 }
 
 // Four channels a workgroup, a thread per partial row: totals, parameter gradients, and the coefficients a, b, c of dx.  The partial sums
 // were written from all over the card: few workgroups with long chains of such reads cost 19 us for 1024 x 256 channels, this 7 us.
-__global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, float inv_rows,
+__global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, int ld, float inv_rows,
                                                            const float* __restrict__ gamma, const float* __restrict__ invstd,
                                                            float* __restrict__ coef, float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                            int accumulate) {
     __shared__ float red[4][8];
     const int tid = threadIdx.x, c0 = blockIdx.x * 4;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};       // sums of d, of d (x8 - mean), four channels each
-    if (c0 + 4 <= C) {
 #pragma unroll 4
-        for (int g = tid; g < groups; g += 256) {
-            const float* p = part + (int64_t)g * 2 * C + c0;
-            const u32x4_t a = *reinterpret_cast<const u32x4_a4*>(p), b = *reinterpret_cast<const u32x4_a4*>(p + C);
+    for (int g = tid; g < groups; g += 256) {
+        const float* p = part + (int64_t)g * 2 * ld + c0;
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p), b = *reinterpret_cast<const u32x4_t*>(p + ld);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { s[j] += __uint_as_float(a[j]); s[4 + j] += __uint_as_float(b[j]); }
-        }
-    } else {
-        for (int g = tid; g < groups; g += 256)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c0 + j < C) { s[j] += part[(int64_t)g * 2 * C + c0 + j]; s[4 + j] += part[((int64_t)g * 2 + 1) * C + c0 + j]; }
+        for (int j = 0; j < 4; ++j) { s[j] += __uint_as_float(a[j]); s[4 + j] += __uint_as_float(b[j]); }
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = wave_sum(s[j]);
@@ -126,8 +120,8 @@ __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restri
         const float s1 = (red[0][4 + tid] + red[1][4 + tid]) + (red[2][4 + tid] + red[3][4 + tid]);
         const float is = invstd[ch], dg = s1 * is, a = gamma[ch] * is;
         coef[ch] = a;
-        coef[C + ch] = a * is * dg * inv_rows;
-        coef[2 * C + ch] = a * s0 * inv_rows;
+        coef[ld + ch] = a * is * dg * inv_rows;
+        coef[2 * ld + ch] = a * s0 * inv_rows;
         dgamma[ch] = accumulate ? dgamma[ch] + dg : dg;
         dbeta[ch] = accumulate ? dbeta[ch] + s0 : s0;
     }
@@ -159,6 +153,11 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
         k.template fix<FULL>();
         k.get(o);
     };
+    auto whole = [&](const float* p, float (&o)[8]) {             // a row of `ld` channels (16-byte aligned)
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(p + c * 8), b = *reinterpret_cast<const u32x4_t*>(p + c * 8 + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { o[j] = __uint_as_float(a[j]); o[4 + j] = __uint_as_float(b[j]); }
+    };
     get(mean, mu);
     if (JOIN) {
         float s0[8], s1[8], is[8], ga[8];
@@ -167,8 +166,8 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
 #pragma unroll 4
         for (int k = 0; k < t.groups; ++k) {
             float a[8], b[8];
-            get(t.part + (int64_t)k * 2 * g.C, a);
-            get(t.part + ((int64_t)k * 2 + 1) * g.C, b);
+            whole(t.part + (int64_t)k * 2 * g.ld, a);
+            whole(t.part + ((int64_t)k * 2 + 1) * g.ld, b);
 #pragma unroll
             for (int j = 0; j < 8; ++j) { s0[j] += a[j]; s1[j] += b[j]; }
         }
@@ -186,9 +185,9 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
             }
         }
     } else {
-        get(t.coef, ka);
-        get(t.coef + g.C, kb);
-        get(t.coef + 2 * g.C, kc);
+        whole(t.coef, ka);
+        whole(t.coef + g.ld, kb);
+        whole(t.coef + 2 * g.ld, kc);
     }
     for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
         MxBnRow<T> row[MXBN_U];
@@ -316,7 +315,7 @@ static int mxbn_groups(int64_t rows, int C) {
 
 extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C) {
     if (rows <= MXBN_SMALL || C < 1 || C > MX_MAX_C) return 0;
-    return sizeof(float) * ((size_t)mxbn_groups(rows, C) * 2 + 3) * (size_t)C;
+    return sizeof(float) * ((size_t)mxbn_groups(rows, C) * 2 + 3) * (size_t)(cdiv(C, 8) * 8);
 }
 
 extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scales, const void* signs, const float* gamma, const float* mean,
@@ -327,6 +326,7 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     CN_CHECK_ARG(dy && codes && scales && gamma && mean && invstd && dx && dgamma && dbeta, "cn_mx_bn_bwd: null pointer");
     CN_CHECK_ARG(dres || !racc, "cn_mx_bn_bwd: racc without dres");
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_bn_bwd: codes must be 16-byte aligned");
+    CN_CHECK_ARG(((uintptr_t)ws & 15) == 0, "cn_mx_bn_bwd: the workspace must be 16-byte aligned");
     if (ws_bytes < cn_mx_bn_bwd_bytes(rows, C) || (!ws && ws_bytes)) {
         cn_set_error("cn_mx_bn_bwd: workspace of %zu bytes needed", cn_mx_bn_bwd_bytes(rows, C));
         return CN_EWORKSPACE;
@@ -340,7 +340,7 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     })
 #define MXBN_COMMA ,
     if (rows <= MXBN_SMALL) {
-        MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 0};
+        MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 0, 0};
         const MxBnTail t{nullptr, nullptr, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, 0, accumulate};
         // four, two or one chunk a workgroup: eight rows a thread at most (two where that is enough)
         g.lg = rows <= 512 ? 2 : (rows <= 1024 ? 1 : 0);
@@ -352,8 +352,9 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     }
     const int groups = mxbn_groups(rows, C);
     float* part = (float*)ws;
-    float* coef = part + (size_t)groups * 2 * C;
-    MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), mxbn_lg(C), 0};
+    const int ld = cdiv(C, 8) * 8;
+    float* coef = part + (size_t)groups * 2 * ld;
+    MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), ld, mxbn_lg(C), 0};
     const int tiles = cdiv(cdiv(C, 8), 1 << g.lg);
     const int nrl = 256 >> g.lg;
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
@@ -363,7 +364,7 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     const MxBnTail t{coef, part, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, groups, accumulate};
     const bool joined = groups <= MXBN_JOIN;
     if (!joined) {
-        mx_bn_finish_kernel<<<cdiv(C, 4), 256, 0, st>>>(part, groups, C, t.inv_rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
+        mx_bn_finish_kernel<<<cdiv(C, 4), 256, 0, st>>>(part, groups, C, ld, t.inv_rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
         CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     }
     // eight rows a thread (its coefficients are loaded once), fewer where that would leave compute units idle

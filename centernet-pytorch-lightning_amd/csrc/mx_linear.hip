@@ -328,12 +328,16 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
 }
+// Which waves do what, us (bf16, M x K x N):
+//   K split over the waves, 32 x 32 a workgroup | columns over the waves, 32 x 256: 1x2048x512 4.5 | -, 64x1440x64 8.8 | 10.3, 512x2048x512
+//     10.9 | 13.0, 2048x64x256 5.1 | 5.5, 20000x1440x8 15.4 | 17.5; the other way 512x512x2048 9.3 | 6.6, 8192x512x64 6.9 | 6.4, 8192x1024x256 15.2 | 10.0
+//   rows over the waves, 128 x 64 | 64 x 128 | 32 x 256: 65536x64x64 7.4 | 8.7 | 11.4, 65536x256x128 16.4 | 13.0 | 14.5, 65536x64x256
+//     13.4 | 12.9 | 14.7, 65536x512x64 17.5 | 17.4 | 16.4, 65536x1024x256 111 | 53 | 45, 65536x256x1024 93 | 71 | 68
 template <typename T, bool FULLK, bool FULLN>
 static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
-    // few rows: less than one 64 x 256 workgroup for each compute unit
-    if ((g.M + 63) / 64 * cdiv(g.N, 256) < 256) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
-    if (g.N <= 64) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
-    if (g.N <= 128) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
+    if (g.N <= 32 || (g.M + 31) / 32 * cdiv(g.N, 32) <= 512) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
+    if (g.N <= 64 && g.K <= 256) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
+    if ((g.N <= 128 && g.K <= 256) || g.K <= 64) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
     return mxl_launch<T, 1, 2, 1, 4, 1, FULLK, FULLN>(g, st);
 }
 
