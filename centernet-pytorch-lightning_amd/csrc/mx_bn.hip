@@ -216,15 +216,16 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
 }
 
 // Few rows: everything in one launch.  A thread keeps its U rows of a chunk in registers between the sums and dx, so a workgroup (all
-// rows of 2^lg chunks) reads its inputs once.  The chunks of a cache line belong to neighbouring workgroups: these are dealt to one XCD.
-template <typename T, bool SIGNS, bool FULL, int U>
-__global__ __launch_bounds__(256) void mx_bn_small_kernel(const MxBnGeom g, const float* __restrict__ mean, const MxBnTail t,
-                                                          T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc, int wgs) {
-    __shared__ float red[4][4 * 16];
+// rows of four chunks) reads its inputs once.  The chunks of a cache line belong to neighbouring workgroups: these are dealt to one XCD.
+template <typename T, bool SIGNS, bool FULL, int U, int NT>
+__global__ __launch_bounds__(NT) void mx_bn_small_kernel(const MxBnGeom g, const float* __restrict__ mean, const MxBnTail t,
+                                                         T* __restrict__ dx, T* __restrict__ dres, const T* __restrict__ racc, int wgs) {
+    constexpr int TC = 4, nrl = NT / TC, NW = NT / 64;
+    __shared__ float red[NW][TC * 16];
     const int per = (wgs + 7) / 8, wg = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || wg >= wgs) return;       // (the grid is 8 x per)
-    const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
-    const int c = wg * tc + cl, left = g.C - c * 8;
+    if (wg >= wgs) return;                                        // (the grid is 8 x per)
+    const int tid = threadIdx.x, cl = tid & (TC - 1), rl = tid / TC;
+    const int c = wg * TC + cl, left = g.C - c * 8;
     MxBnRow<T> row[U];
     float mu[8], s0[8], s1[8];
     auto get = [&](const float* p, float (&o)[8]) {
@@ -247,13 +248,23 @@ __global__ __launch_bounds__(256) void mx_bn_small_kernel(const MxBnGeom g, cons
             for (int j = 0; j < 8; ++j) { s0[j] += d[j]; s1[j] = fmaf(d[j], v[j] - mu[j], s1[j]); }
         }
     }
-    for (int o = 32; o >= tc; o >>= 1) {
+    // sixteen lanes hold a chunk's sixteen sums each: every step adds half of what is left over a pair of lanes (15 moves, not 64)
+    float r8[8], r4[4], r2[2];
+    const bool b5 = tid & 32, b4 = tid & 16, b3 = tid & 8, b2 = tid & 4;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { s0[j] += __shfl_xor(s0[j], o, 64); s1[j] += __shfl_xor(s1[j], o, 64); }
-    }
-    if ((tid & 63) < tc) {
+    for (int j = 0; j < 8; ++j) r8[j] = (b5 ? s1[j] : s0[j]) + __shfl_xor(b5 ? s0[j] : s1[j], 32, 64);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { red[tid >> 6][cl * 16 + j] = s0[j]; red[tid >> 6][cl * 16 + 8 + j] = s1[j]; }
+    for (int j = 0; j < 4; ++j) r4[j] = (b4 ? r8[4 + j] : r8[j]) + __shfl_xor(b4 ? r8[j] : r8[4 + j], 16, 64);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) r2[j] = (b3 ? r4[2 + j] : r4[j]) + __shfl_xor(b3 ? r4[j] : r4[2 + j], 8, 64);
+    const float r1 = (b2 ? r2[1] : r2[0]) + __shfl_xor(b2 ? r2[0] : r2[1], 4, 64);
+    red[tid >> 6][cl * 16 + (b5 ? 8 : 0) + (b4 ? 4 : 0) + (b3 ? 2 : 0) + (b2 ? 1 : 0)] = r1;
+    __syncthreads();
+    if (tid < TC * 16) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += red[w][tid];
+        red[0][tid] = v;                                          // (each thread has its own column)
     }
     __syncthreads();
     if (left <= 0) return;
@@ -262,8 +273,7 @@ __global__ __launch_bounds__(256) void mx_bn_small_kernel(const MxBnGeom g, cons
     get(t.gamma, ga);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const int a = cl * 16 + j, b = a + 8;
-        const float t0 = (red[0][a] + red[1][a]) + (red[2][a] + red[3][a]), t1 = (red[0][b] + red[1][b]) + (red[2][b] + red[3][b]);
+        const float t0 = red[0][cl * 16 + j], t1 = red[0][cl * 16 + 8 + j];
         const float dg = t1 * is[j];
         ka[j] = ga[j] * is[j];
         kb[j] = ka[j] * is[j] * dg * t.inv_rows;
@@ -295,7 +305,9 @@ __global__ __launch_bounds__(256) void mx_bn_small_kernel(const MxBnGeom g, cons
     }
 }
 
-#define MXBN_SMALL 2048        // rows that 256 threads hold eight of each
+// rows of four chunks that a workgroup holds.  us, one launch | two or three: 128x512 5.3 | 10, 512x512 7.2 | 11, 700x512 8.3 | 11.6; eight rows
+// a thread for 2048 rows: 1471x30 16 | 10.2
+#define MXBN_SMALL 1024
 
 static int mxbn_lg(int C) {
     const int chunks = cdiv(C, 8);
@@ -313,7 +325,7 @@ static int mxbn_groups(int64_t rows, int C) {
     return (int)(g < 1 ? 1 : (g > MXBN_MAX_GROUPS ? MXBN_MAX_GROUPS : g));
 }
 
-extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C) {
+extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C, int dtype) {
     if (rows <= MXBN_SMALL || C < 1 || C > MX_MAX_C) return 0;
     return sizeof(float) * ((size_t)mxbn_groups(rows, C) * 2 + 3) * (size_t)(cdiv(C, 8) * 8);
 }
@@ -327,8 +339,8 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     CN_CHECK_ARG(dres || !racc, "cn_mx_bn_bwd: racc without dres");
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_bn_bwd: codes must be 16-byte aligned");
     CN_CHECK_ARG(((uintptr_t)ws & 15) == 0, "cn_mx_bn_bwd: the workspace must be 16-byte aligned");
-    if (ws_bytes < cn_mx_bn_bwd_bytes(rows, C) || (!ws && ws_bytes)) {
-        cn_set_error("cn_mx_bn_bwd: workspace of %zu bytes needed", cn_mx_bn_bwd_bytes(rows, C));
+    if (ws_bytes < cn_mx_bn_bwd_bytes(rows, C, dtype) || (!ws && ws_bytes)) {
+        cn_set_error("cn_mx_bn_bwd: workspace of %zu bytes needed", cn_mx_bn_bwd_bytes(rows, C, dtype));
         return CN_EWORKSPACE;
     }
     hipStream_t st = (hipStream_t)stream;
@@ -340,13 +352,18 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     })
 #define MXBN_COMMA ,
     if (rows <= MXBN_SMALL) {
-        MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 0, 0};
+        const MxBnGeom g{dy, (const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)signs, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 0, 0};
         const MxBnTail t{nullptr, nullptr, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, 0, accumulate};
-        // four, two or one chunk a workgroup: eight rows a thread at most (two where that is enough)
-        g.lg = rows <= 512 ? 2 : (rows <= 1024 ? 1 : 0);
-        const int wgs = cdiv(cdiv(C, 8), 1 << g.lg), grid = cdiv(wgs, 8) * 8;
-        if (rows <= 2 * (256 >> g.lg)) MXBN_GO(mx_bn_small_kernel, MXBN_COMMA 2, grid, g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs);
-        else MXBN_GO(mx_bn_small_kernel, MXBN_COMMA 8, grid, g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs);
+        const int wgs = cdiv(cdiv(C, 8), 4), grid = cdiv(wgs, 8) * 8;
+#define MXBN_SMALL_GO(T, S, U, NT)                                                                                                     \
+    do { if (full) mx_bn_small_kernel<T, S, true, U, NT><<<grid, NT, 0, st>>>(g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs);      \
+         else mx_bn_small_kernel<T, S, false, U, NT><<<grid, NT, 0, st>>>(g, mean, t, (T*)dx, (T*)dres, (const T*)racc, wgs); } while (0)
+#define MXBN_SMALL_ROWS(T, S)                                                                                                          \
+    do { if (rows <= 128) MXBN_SMALL_GO(T, S, 2, 256); else if (rows <= 512) MXBN_SMALL_GO(T, S, 2, 1024); else MXBN_SMALL_GO(T, S, 4, 1024); } while (0)
+        if (dtype == CN_BF16) { if (signs) MXBN_SMALL_ROWS(bf16_t, true); else MXBN_SMALL_ROWS(bf16_t, false); }
+        else { if (signs) MXBN_SMALL_ROWS(float, true); else MXBN_SMALL_ROWS(float, false); }
+#undef MXBN_SMALL_ROWS
+#undef MXBN_SMALL_GO
         CN_LAUNCH_CHECK("cn_mx_bn_bwd");
         return CN_OK;
     }

@@ -95,28 +95,48 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
     auto stage = [&](int s0, int s1) {
         const MxDiv dv = s1 == g.S ? g.div_last : g.div_full;
         const int total = rows * (int)dv.d;
-        constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;            // loads in flight per thread
-        for (int base = tid; base < total; base += 256 * U) {
-            MxRaw8<T> v[U];
-            int row[U], pc[U];
+        constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;            // loads in flight per thread; WK > 1: and as many again
+        struct Batch { MxRaw8<T> v[U]; int row[U], pc[U]; };
+        auto ask = [&](Batch& q, int base) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const uint32_t i = base + u * 256;
-                row[u] = (int)mx_quot(i, dv);
-                pc[u] = (int)i - row[u] * (int)dv.d;
-                const int c0 = s0 * 64 + pc[u] * 8;
-                v[u].template load<FULLK>(X, (int64_t)row[u] * g.K + c0, g.K - c0, (int)i < total, g.K);
+                q.row[u] = (int)mx_quot(i, dv);
+                q.pc[u] = (int)i - q.row[u] * (int)dv.d;
+                const int c0 = s0 * 64 + q.pc[u] * 8;
+                q.v[u].template load<FULLK>(X, (int64_t)q.row[u] * g.K + c0, g.K - c0, (int)i < total, g.K);
             }
+        };
+        auto take = [&](Batch& q, int base) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 float f[8];
-                v[u].template fix<FULLK>();
-                v[u].get(f);
+                q.v[u].template fix<FULLK>();
+                q.v[u].get(f);
                 const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(mx_absmax8(f)));
                 if (base + u * 256 < total) {                     // (whole quads)
-                    *reinterpret_cast<uint32_t*>(smem + row[u] * g.pitch + pc[u] * 4) = mx_codes_e2m1(f, b);
-                    const int blk = pc[u] >> 2, s = blk >> 1;     // byte s & 3 of word (s / 4, half)
-                    if ((pc[u] & 3) == 0) smem[g.sc_ofs + row[u] * g.spitch + ((s >> 2) * 2 + (blk & 1)) * 4 + (s & 3)] = (uint8_t)b;
+                    *reinterpret_cast<uint32_t*>(smem + q.row[u] * g.pitch + q.pc[u] * 4) = mx_codes_e2m1(f, b);
+                    const int blk = q.pc[u] >> 2, s = blk >> 1;   // byte s & 3 of word (s / 4, half)
+                    if ((q.pc[u] & 3) == 0) smem[g.sc_ofs + q.row[u] * g.spitch + ((s >> 2) * 2 + (blk & 1)) * 4 + (s & 3)] = (uint8_t)b;
+                }
+            }
+        };
+        if (WK == 1) {
+            for (int base = tid; base < total; base += 256 * U) {
+                Batch q;
+                ask(q, base);
+                take(q, base);
+            }
+        } else {
+            Batch q, r;
+            ask(q, tid);
+            for (int base = tid; base < total; base += 512 * U) {
+                const bool more = base + 256 * U < total;
+                if (more) ask(r, base + 256 * U);
+                take(q, base);
+                if (more) {
+                    if (base + 512 * U < total) ask(q, base + 512 * U);
+                    take(r, base + 256 * U);
                 }
             }
         }

@@ -342,8 +342,9 @@ extern "C" int cn_mx_linear_wgrad(const void* dy, const void* codes, const void*
     if (join) {
         const int64_t n = (int64_t)N * K;
         const int nb = db ? N : 0;
-        // sixteen groups where the splits are many and the outputs few; 64 / 1024 outputs a workgroup
-        if (p.splits >= 16) mx_wgrad_join_kernel<16><<<(unsigned)(cdiv(n, 64) + cdiv(nb, 64)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        // more groups where the splits are many and the outputs few; 16 / 64 / 1024 outputs a workgroup
+        if (p.splits >= 128 && n <= 4096) mx_wgrad_join_kernel<64><<<(unsigned)(cdiv(n, 16) + cdiv(nb, 16)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        else if (p.splits >= 16) mx_wgrad_join_kernel<16><<<(unsigned)(cdiv(n, 64) + cdiv(nb, 64)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         else mx_wgrad_join_kernel<1><<<(unsigned)(cdiv(n, 1024) + cdiv(nb, 1024)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
     }

@@ -272,7 +272,7 @@ def batch_norm_act_bwd(dy, ck, gamma, mean, invstd, residual=False, racc=None, i
         dgamma, dbeta = torch.empty(one, dtype=torch.float32, device=dev), torch.empty(one, dtype=torch.float32, device=dev)
     dx = torch.empty_like(dy)
     dres = torch.empty_like(dy) if residual else None
-    n = _hip.query("cn_mx_bn_bwd_bytes", rows, C)
+    n = _hip.query("cn_mx_bn_bwd_bytes", rows, C, dt)
     ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     codes, scales, signs = ck._pointers()
     launch("cn_mx_bn_bwd", dy.get_device(), dy.data_ptr(), codes, scales, signs, gamma.data_ptr(), mean.data_ptr(), invstd.data_ptr(),

@@ -562,7 +562,7 @@ int cn_mx_linear_wgrad(const void* dy, const void* codes, const void* scales, fl
                        int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream);
 /* backward of y = [relu](gamma * (x - mean) * invstd + beta [+ residual]) with batch statistics, from an e4m3 checkpoint of x; signs:
  * the ReLU's sign bits (null: no ReLU).  dres (may be null): gradient of the residual input, plus racc (may be null). */
-size_t cn_mx_bn_bwd_bytes(int64_t rows, int C);
+size_t cn_mx_bn_bwd_bytes(int64_t rows, int C, int dtype);
 int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scales, const void* signs, const float* gamma, const float* mean,
                  const float* invstd, void* dx, void* dres, const void* racc, float* dgamma, float* dbeta, int accumulate,
                  int64_t rows, int C, int dtype, void* ws, size_t ws_bytes, void* stream);

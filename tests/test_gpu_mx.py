@@ -301,7 +301,7 @@ def test_linear_wgrad_refusals():
 
 
 # ------------------------------------------------------------------------------------------------ batch norm
-NORM = [(2, 1), (3, 8), (5, 33), (64, 80), (300, 64), (129, 515), (2000, 256), (7, 2048), (30000, 16), (11, 4100), (512, 100), (1024, 24), (2048, 72),
+NORM = [(2, 1), (3, 8), (5, 33), (64, 80), (300, 64), (129, 515), (2000, 256), (7, 2048), (30000, 16), (11, 4100), (512, 100), (513, 24), (1024, 24), (1025, 72),
         (2049, 72), (2100, 13), (9000, 520), (70000, 7)]
 
 

@@ -66,10 +66,10 @@ def test_entry_points_ask_for_workspace(lib):
     assert n > 4 * 64 * 64
     assert lib.cn_mx_linear_wgrad(P, P, P, P, None, 0, 100000, 64, 64, 1, P, n - 1, None) == -3
     assert lib.cn_mx_linear_wgrad(P, P, P, P, None, 0, 100000, 64, 64, 1, None, n, None) == -3
-    n = lib.cn_mx_bn_bwd_bytes(100000, 64)
+    n = lib.cn_mx_bn_bwd_bytes(100000, 64, 1)
     assert n > 4 * 64
     assert lib.cn_mx_bn_bwd(P, P, P, None, P, P, P, P, None, None, P, P, 0, 100000, 64, 1, P, n - 1, None) == -3
-    for bad in ((0, 64), (8, 0), (8, 65537)):
+    for bad in ((0, 64, 1), (100000, 0, 1), (100000, 65537, 0)):
         assert lib.cn_mx_bn_bwd_bytes(*bad) == 0
     assert lib.cn_mx_weight_bytes(0, 8) == 0 and lib.cn_mx_weight_bytes(8, 70000) == 0
     assert lib.cn_mx_weight_bytes(33, 65) == 2 * 2 * 1024 + 2 * 256
