@@ -20,7 +20,7 @@ struct MxBnGeom {
     int C, cpr, blocks;        // cpr: 8-channel chunks per (padded) row of codes, blocks = cpr / 4
     int ld;                    // C rounded up to 8: channels per row of the partial sums and of the coefficients
     int lg;                    // log2 of the chunks a workgroup covers
-    int64_t per;               // rows per workgroup
+    int64_t per;               // rows per workgroup of the apply pass
 };
 
 #define MXBN_U 4               // rows a thread has in flight
@@ -49,23 +49,25 @@ template <typename T> struct MxBnRow {
     }
 };
 
+// The workgroups walk the rows side by side (in step with time), and the apply pass starts at the end: what was read last is still in the
+// memory-side cache (45 -> 40 us and 76 -> 74 us at 262144 x 256).
 template <typename T, bool SIGNS, bool FULL>
 __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const float* __restrict__ mean, float* __restrict__ part) {
     __shared__ float red[4 * 32 * 16];
     const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
     const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
-    const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
     float s0[8], s1[8], mu[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; mu[j] = j < left ? mean[c * 8 + j] : 0.f; }
     if (left > 0) {
-        for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
+        for (int64_t r = (int64_t)blockIdx.x * (MXBN_U * nrl) + rl; r < g.rows; r += (int64_t)gridDim.x * (MXBN_U * nrl)) {
             MxBnRow<T> row[MXBN_U];
 #pragma unroll
-            for (int u = 0; u < MXBN_U; ++u) row[u].template load<SIGNS, FULL>(g, r + u * nrl, c, left, r + u * nrl < r1);
+            for (int u = 0; u < MXBN_U; ++u) row[u].template load<SIGNS, FULL>(g, r + u * nrl, c, left, r + u * nrl < g.rows);
+            MX_LOADS_OUT();
 #pragma unroll
             for (int u = 0; u < MXBN_U; ++u) {
-                if (r + u * nrl < r1) {
+                if (r + u * nrl < g.rows) {
                     float d[8], v[8];
                     row[u].template get<SIGNS, FULL>(d, v);
 #pragma unroll
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
     const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
     const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
     if (left <= 0) return;
-    const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
+    const int64_t r0 = (int64_t)(gridDim.x - 1 - blockIdx.x) * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
     float ka[8], kb[8], kc[8], mu[8];
     auto get = [&](const float* p, float (&o)[8]) {
         MxRaw8<float> k;
@@ -193,6 +195,7 @@ __global__ __launch_bounds__(256) void mx_bn_apply_kernel(const MxBnGeom g, cons
         MxBnRow<T> row[MXBN_U];
 #pragma unroll
         for (int u = 0; u < MXBN_U; ++u) row[u].template load<SIGNS, FULL>(g, r + u * nrl, c, left, r + u * nrl < r1);
+        MX_LOADS_OUT();
 #pragma unroll
         for (int u = 0; u < MXBN_U; ++u) {
             if (r + u * nrl < r1) {
@@ -236,6 +239,7 @@ __global__ __launch_bounds__(NT) void mx_bn_small_kernel(const MxBnGeom g, const
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) row[u].template load<SIGNS, FULL>(g, rl + u * nrl, left > 0 ? c : 0, left, left > 0 && rl + u * nrl < g.rows);
+    MX_LOADS_OUT();
     get(mean, mu);
 #pragma unroll
     for (int j = 0; j < 8; ++j) { s0[j] = 0.f; s1[j] = 0.f; }
@@ -375,7 +379,6 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     const int tiles = cdiv(cdiv(C, 8), 1 << g.lg);
     const int nrl = 256 >> g.lg;
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
-    g.per = (rows + groups - 1) / groups;
     MXBN_GO(mx_bn_sums_kernel, , dim3(groups, tiles), g, mean, part);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     const MxBnTail t{coef, part, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, groups, accumulate};

@@ -14,6 +14,7 @@
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 // 16 bytes at any 2- / 4-byte aligned address: rows of an odd number of channels start anywhere, and the hardware loads and stores
 // such vectors in one instruction all the same
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -83,6 +84,32 @@ __device__ static inline void mx_store8(bf16_t* p, int left, const float (&v)[8]
     }
 }
 
+__device__ static inline uint32_t mx_absmax8(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; m = a > m ? a : m; }
+    return m;
+}
+// codes of eight values on scale byte b (255: zeros); e2m1 -> 4 bytes, e4m3 -> 8 bytes.  Both conversions round to nearest even, and
+// the scale is an exact power of two: one rounding in all.
+__device__ static inline uint32_t mx_codes_e2m1(const float (&v)[8], uint32_t b) {
+    const float s = mx_scale_value(b);
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
+    return b == 255u ? 0u : r;
+}
+__device__ static inline uint2 mx_codes_e4m3(const float (&v)[8], uint32_t b) {
+    const float s = b == 255u ? 0.f : mx_scale_inverse(b);
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * s, v[1] * s, lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * s, v[3] * s, lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * s, v[5] * s, hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * s, v[7] * s, hi, true);
+    return b == 255u ? make_uint2(0u, 0u) : make_uint2((uint32_t)lo, (uint32_t)hi);
+}
 // Eight consecutive elements as they lie in memory, so that several loads can be in flight before the first is unpacked (an exec-masked
 // branch would make the compiler wait for every load before the next: these have none).  `left`: channels of the row from here on (may
 // be <= 0), `ok`: the row exists; what is not there reads as zero.  FULL: the row has a multiple of 8 channels, so a chunk lies inside
@@ -91,6 +118,8 @@ __device__ static inline void mx_store8(bf16_t* p, int left, const float (&v)[8]
 // A load leaves raw bits and what is wrong with them (s: elements to shift down, 8: nothing was there); `fix` puts that right, at the time
 // of use — done at once it would make every load wait for the one before.
 __device__ static inline u32x4_t mx_pick(bool c, u32x4_t a, u32x4_t b) { return u32x4_t{c ? a.x : b.x, c ? a.y : b.y, c ? a.z : b.z, c ? a.w : b.w}; }
+// MX_LOADS_OUT() ends a batch of loads: without it the scheduler moves a first use between them, and its wait with it.
+#define MX_LOADS_OUT() __builtin_amdgcn_sched_barrier(0)
 template <typename T> struct MxRaw8;
 template <> struct MxRaw8<bf16_t> {
     u32x4_t a;
@@ -121,6 +150,18 @@ template <> struct MxRaw8<bf16_t> {
     __device__ inline void get(float (&f)[8]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(a[i] << 16); f[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u); }
+    }
+    // bits (as float) of the largest magnitude: the order of the 16-bit magnitudes is theirs
+    __device__ inline uint32_t absmax() const {
+        u16x2_t m = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, a[i] & 0x7fff7fffu));
+        return (uint32_t)(m.x > m.y ? m.x : m.y) << 16;
+    }
+    __device__ inline uint32_t codes_e2m1(uint32_t scale) const {
+        float f[8];
+        get(f);
+        return mx_codes_e2m1(f, scale);
     }
 };
 template <> struct MxRaw8<float> {
@@ -162,6 +203,16 @@ template <> struct MxRaw8<float> {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { f[i] = __uint_as_float(a[i]); f[4 + i] = __uint_as_float(b[i]); }
     }
+    __device__ inline uint32_t absmax() const {
+        float f[8];
+        get(f);
+        return mx_absmax8(f);
+    }
+    __device__ inline uint32_t codes_e2m1(uint32_t scale) const {
+        float f[8];
+        get(f);
+        return mx_codes_e2m1(f, scale);
+    }
 };
 // store of eight elements of such a row (FULL as above)
 template <bool FULL, typename T> __device__ static inline void mx_store8f(T* p, int left, const float (&v)[8]) {
@@ -169,32 +220,6 @@ template <bool FULL, typename T> __device__ static inline void mx_store8f(T* p, 
     else mx_store8(p, left, v);
 }
 
-__device__ static inline uint32_t mx_absmax8(const float (&v)[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu; m = a > m ? a : m; }
-    return m;
-}
-// codes of eight values on scale byte b (255: zeros); e2m1 -> 4 bytes, e4m3 -> 8 bytes.  Both conversions round to nearest even, and
-// the scale is an exact power of two: one rounding in all.
-__device__ static inline uint32_t mx_codes_e2m1(const float (&v)[8], uint32_t b) {
-    const float s = mx_scale_value(b);
-    uint32_t r = 0;
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], s, 0);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], s, 1);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], s, 2);
-    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], s, 3);
-    return b == 255u ? 0u : r;
-}
-__device__ static inline uint2 mx_codes_e4m3(const float (&v)[8], uint32_t b) {
-    const float s = b == 255u ? 0.f : mx_scale_inverse(b);
-    int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * s, v[1] * s, lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * s, v[3] * s, lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * s, v[5] * s, hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * s, v[7] * s, hi, true);
-    return b == 255u ? make_uint2(0u, 0u) : make_uint2((uint32_t)lo, (uint32_t)hi);
-}
 // the eight values that 8 bytes of e4m3 codes stand for
 __device__ static inline void mx_values_e4m3(uint32_t lo, uint32_t hi, float s, float (&v)[8]) {
     f32x2_t p = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false); v[0] = p.x * s; v[1] = p.y * s;

@@ -72,7 +72,6 @@ struct MxLinGeom {
     int per_wg;                // passes over the workgroup's columns
     int relu;
     int pitch, spitch;         // LDS bytes per row: codes, scales
-    MxDiv div_full, div_last;  // 8-channel pieces per row of a full / the last chunk
     int sc_ofs, ep_ofs;        // LDS offsets of the scales and of the output staging
 };
 
@@ -91,52 +90,61 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
     const int rows = (int)(g.M - m0 < BM ? g.M - m0 : BM);
     const T* __restrict__ X = reinterpret_cast<const T*>(g.x) + m0 * g.K;
 
-    // quantise channels 64 s0 .. 64 s1 of the workgroup's rows into LDS (rows behind the last stay as they are: what they give is not stored)
+    // Quantise channels 64 s0 .. 64 s1 of the workgroup's rows into LDS (rows behind the last stay as they are: what they give is not
+    // stored).  A thread's chunks are 256 apart; row and channel are carried along (multiplications cost four times an addition).
     auto stage = [&](int s0, int s1) {
-        const MxDiv dv = s1 == g.S ? g.div_last : g.div_full;
-        const int total = rows * (int)dv.d;
-        constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;            // loads in flight per thread; WK > 1: and as many again
-        struct Batch { MxRaw8<T> v[U]; int row[U], pc[U]; };
-        auto ask = [&](Batch& q, int base) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t i = base + u * 256;
-                q.row[u] = (int)mx_quot(i, dv);
-                q.pc[u] = (int)i - q.row[u] * (int)dv.d;
-                const int c0 = s0 * 64 + q.pc[u] * 8;
-                q.v[u].template load<FULLK>(X, (int64_t)q.row[u] * g.K + c0, g.K - c0, (int)i < total, g.K);
-            }
+        const int d = (s1 - s0) * 8, dq = 256 / d, dr = 256 - dq * d;          // 8-channel chunks per row (uniform)
+        const uint32_t step = (uint32_t)(dq * g.K + dr * 8), wrap = (uint32_t)(g.K - d * 8);
+        constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;                   // loads in flight per thread; WK > 1: and as many again
+        struct At { int row, pc; uint32_t ofs; };
+        auto next = [&](At& t) {
+            t.row += dq;
+            t.pc += dr;
+            t.ofs += step;
+            if (t.pc >= d) { t.pc -= d; t.row += 1; t.ofs += wrap; }
         };
-        auto take = [&](Batch& q, int base) {
+        struct Batch { MxRaw8<T> v[U]; };
+        auto ask = [&](Batch& q, At& t) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float f[8];
+                q.v[u].template load<FULLK>(X, t.ofs, g.K - s0 * 64 - t.pc * 8, t.row < rows, g.K);
+                next(t);
+            }
+            MX_LOADS_OUT();
+        };
+        auto take = [&](Batch& q, At& t) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
                 q.v[u].template fix<FULLK>();
-                q.v[u].get(f);
-                const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(mx_absmax8(f)));
-                if (base + u * 256 < total) {                     // (whole quads)
-                    *reinterpret_cast<uint32_t*>(smem + q.row[u] * g.pitch + q.pc[u] * 4) = mx_codes_e2m1(f, b);
-                    const int blk = q.pc[u] >> 2, s = blk >> 1;   // byte s & 3 of word (s / 4, half)
-                    if ((q.pc[u] & 3) == 0) smem[g.sc_ofs + q.row[u] * g.spitch + ((s >> 2) * 2 + (blk & 1)) * 4 + (s & 3)] = (uint8_t)b;
+                const uint32_t b = mx_scale_byte<CN_MX_E2M1>(quad_max_u(q.v[u].absmax()));
+                if (t.row < rows) {                               // (whole quads)
+                    *reinterpret_cast<uint32_t*>(smem + t.row * g.pitch + t.pc * 4) = q.v[u].codes_e2m1(b);
+                    const int blk = t.pc >> 2, s = blk >> 1;      // byte s & 3 of word (s / 4, half)
+                    if ((t.pc & 3) == 0) smem[g.sc_ofs + t.row * g.spitch + ((s >> 2) * 2 + (blk & 1)) * 4 + (s & 3)] = (uint8_t)b;
                 }
+                next(t);
             }
         };
+        At t0;
+        t0.row = tid / d;
+        t0.pc = tid - t0.row * d;
+        t0.ofs = (uint32_t)(t0.row * g.K + s0 * 64 + t0.pc * 8);
+        At t1 = t0;
         if (WK == 1) {
-            for (int base = tid; base < total; base += 256 * U) {
+            while (t1.row < rows) {
                 Batch q;
-                ask(q, base);
-                take(q, base);
+                ask(q, t0);
+                take(q, t1);
             }
         } else {
             Batch q, r;
-            ask(q, tid);
-            for (int base = tid; base < total; base += 512 * U) {
-                const bool more = base + 256 * U < total;
-                if (more) ask(r, base + 256 * U);
-                take(q, base);
-                if (more) {
-                    if (base + 512 * U < total) ask(q, base + 512 * U);
-                    take(r, base + 256 * U);
+            ask(q, t0);
+            while (t1.row < rows) {
+                if (t0.row < rows) ask(r, t0);
+                take(q, t1);
+                if (t1.row < rows) {
+                    if (t0.row < rows) ask(q, t0);
+                    take(r, t1);
                 }
             }
         }
@@ -215,6 +223,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
                 const int64_t m = m0 + wm * MI * 32 + q * RPI + lane / LPR;
                 rv[q].template load<FULLN>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M, g.N);
             }
+            MX_LOADS_OUT();
         }
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -323,8 +332,6 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     g.sc_ofs = BM * g.pitch;
     g.ep_ofs = (BM * (g.pitch + g.spitch) + 15) / 16 * 16;
     const int smem = g.ep_ofs + ep;
-    g.div_full = mx_div((uint32_t)chunk * 8);
-    g.div_last = mx_div((uint32_t)(g.S % chunk ? g.S % chunk : chunk) * 8);
     g.t32 = cdiv(g.N, 32);
     const int64_t mt = (g.M + BM - 1) / BM;
     if (mt >= ((int64_t)1 << 31)) { cn_set_error("cn_mx_linear_fwd: too many rows"); return CN_EINVAL; }

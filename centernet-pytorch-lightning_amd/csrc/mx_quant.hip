@@ -22,16 +22,20 @@ __global__ __launch_bounds__(256) void mx_quantize_kernel(const T* __restrict__ 
         v[u].template load<FULL>(x, at, C - c0, base + l < chunks, C);
         if (SIGNS) w[u].template load<FULL>(sg, at, C - c0, base + l < chunks, C);
     }
+    MX_LOADS_OUT();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t i = base + threadIdx.x + u * 256;
         if (i >= chunks) return;                                         // (chunks is a multiple of 4: a quad stays whole)
-        float f[8];
         v[u].template fix<FULL>();
-        v[u].get(f);
-        const uint32_t b = mx_scale_byte<FMT>(quad_max_u(mx_absmax8(f)));
-        if (FMT == CN_MX_E2M1) reinterpret_cast<uint32_t*>(codes)[i] = mx_codes_e2m1(f, b);
-        else reinterpret_cast<uint2*>(codes)[i] = mx_codes_e4m3(f, b);
+        const uint32_t b = mx_scale_byte<FMT>(quad_max_u(v[u].absmax()));
+        if (FMT == CN_MX_E2M1) {
+            reinterpret_cast<uint32_t*>(codes)[i] = v[u].codes_e2m1(b);
+        } else {
+            float f[8];
+            v[u].get(f);
+            reinterpret_cast<uint2*>(codes)[i] = mx_codes_e4m3(f, b);
+        }
         if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)b;
         if (SIGNS) {
             float s[8];

@@ -7,7 +7,8 @@ for serving, and the backward passes that read 8-bit activation checkpoints.
                                            dx, dgamma, dbeta, dres = mx.batch_norm_act_bwd(dy, ck, gamma, mean, invstd)
 
 Tensors are [..., channels] in torch.bfloat16 or torch.float32 (NHWC activations of the other operators, or rows of a linear layer);
-any channel count from 1 to 65536 and any number of rows, zero included where a result is defined.  Non-contiguous inputs are copied.
+any channel count from 1 to 65536 and any number of rows, zero included where a result is defined.  Nothing here is recorded by autograd
+(the layers' autograd functions call these).  Non-contiguous inputs are copied.
 Work is enqueued on the current stream of the tensors' device; nothing synchronises and scratch comes from torch's allocator, so every
 call can be captured into a graph and two captured graphs share no scratch.  Results do not depend on the launch (sums have a fixed
 order).  Layers use these operators through `nn.use_checkpoints` (training) and `nn.use_mxfp4` (no-grad forward).
@@ -268,6 +269,8 @@ def batch_norm_act_bwd(dy, ck, gamma, mean, invstd, residual=False, racc=None, i
         for t in into:
             if _like(t, dev, one, torch.float32, "mx.batch_norm_act_bwd: into") is not t:
                 raise ValueError("mx.batch_norm_act_bwd: into must be contiguous")
+        if dgamma.data_ptr() == dbeta.data_ptr():
+            raise ValueError("mx.batch_norm_act_bwd: into needs two tensors")
     else:
         dgamma, dbeta = torch.empty(one, dtype=torch.float32, device=dev), torch.empty(one, dtype=torch.float32, device=dev)
     dx = torch.empty_like(dy)

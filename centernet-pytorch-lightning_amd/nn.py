@@ -103,7 +103,9 @@ class Conv2d(nn.Module):
                     b[:Co] = self.bias if scale is None else self.bias * scale
                 if shift is not None:
                     b[:Co] += shift
-            hit = self._mx_cache = (key, mx.pack_weight(w), b)
+            hit = (key, mx.pack_weight(w), b)
+            if not torch.cuda.is_current_stream_capturing():       # (what a capture packs exists only once the graph has run)
+                self._mx_cache = hit
         return hit[1], hit[2]
 
     def infer_nchw(self, x):

@@ -110,6 +110,15 @@ def test_quantise_any_address_and_order(dt, C):
     same_quantised(q, x, "e4m3")
 
 
+def test_one_dimension():
+    m, x, w = mx(), rnd((96,), 1, BF, spread=0), rnd((40, 96), 2, F32)
+    same_quantised(m.quantize(x, "e4m3"), x, "e4m3")
+    assert m.dequantize(m.quantize(x, "e2m1")).shape == (96,)
+    assert torch.equal(m.linear(x, m.pack_weight(w)), m.linear(x.view(1, 96), m.pack_weight(w))[0])
+    dy = rnd((40,), 3, BF, spread=0)
+    assert torch.equal(m.linear_wgrad(dy, m.checkpoint(x))[0], m.linear_wgrad(dy.view(1, 40), m.checkpoint(x.view(1, 96)))[0])
+
+
 def test_dequantise_writes_its_rows_only():
     x = rnd((7, 77), 3, BF)
     q = mx().quantize(x, "e4m3")
@@ -350,7 +359,8 @@ def test_batch_norm_refusals():
                 lambda: m.batch_norm_act_bwd(dy, ck, v[:31], v, v), lambda: m.batch_norm_act_bwd(dy, ck, v, v.to(BF), v),
                 lambda: m.batch_norm_act_bwd(dy, ck, v, v, v, racc=dy), lambda: m.batch_norm_act_bwd(dy, ck, v, v, v.cpu()),
                 lambda: m.batch_norm_act_bwd(dy, ck, v, v, v, residual=True, racc=dy[:5]),
-                lambda: m.batch_norm_act_bwd(dy, ck, v, v, v, into=(v, torch.ones(64, device=DEV)[::2]))):
+                lambda: m.batch_norm_act_bwd(dy, ck, v, v, v, into=(v, torch.ones(64, device=DEV)[::2])),
+                lambda: m.batch_norm_act_bwd(dy, ck, v, v, v, into=(v, v))):
         with pytest.raises(ValueError):
             bad()
 

@@ -273,6 +273,26 @@ def test_root_and_head_inference_in_4_bits():
         within(y.permute(0, 2, 3, 1).reshape(-1, 20), want, half_step(BF) * np.abs(want) + 72 * U * m, "head")
 
 
+def test_inference_captured_before_any_eager_call():
+    """weights packed during a capture are not kept for eager calls (they hold nothing until the graph has run)"""
+    n = hnn()
+    conv = n.Conv2d(64, 64, 1).to(DEV)
+    x = img((2, 8, 8, 64), 1, BF)
+    n.use_mxfp4(conv)
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = conv(x)
+        eager = conv(x)
+        for _ in range(3):
+            y.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+            assert torch.equal(conv(x), eager)
+
+
 def test_model_inference_in_4_bits():
     """the whole detector: only the 1x1 layers of the backbone change, the maps stay finite and keep their shapes, and switching back
     gives the first result"""
