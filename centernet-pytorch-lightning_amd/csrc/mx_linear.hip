@@ -78,12 +78,13 @@ struct MxLinGeom {
 // two steps of NJ weight tiles
 template <int NJ> struct MxLinB { u32x4_t f[2][NJ]; };
 
-// MI x NJ tiles of 32 x 32 per wave; WM x WN waves over rows and columns, WK over the channels (few rows: the launch would be short of
-// waves otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows
-template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN, bool resident>
+// 32 x 32 NJ outputs per wave; WM x WN waves over rows and columns, WK over the channels (few rows: the launch would be short of waves
+// otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows.  RT > 1 (K <= 256): a wave takes
+// RT row tiles one after the other with the weights of its columns in registers (read from L2 half as often: 65536x256x1024 69 -> 63 us).
+template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN, bool resident>
 __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
-    static_assert(WM * WN * WK == 4 && (WK == 1 || (WK == 4 && MI == 1)), "four waves");
-    constexpr int BM = 32 * MI * WM, EPN = 32 * NJ, EPP = EPN + 4;         // EPP: floats per staged output row (rows on different banks)
+    static_assert(WM * WN * WK == 4 && (WK == 1 || WK == 4) && (RT == 1 || (WK == 1 && resident)), "four waves");
+    constexpr int BM = 32 * RT * WM, EPN = 32 * NJ, EPP = EPN + 4;         // EPP: floats per staged output row (rows on different banks)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = WK > 1 ? 0 : wave / WN, wn = WK > 1 ? 0 : wave % WN, wk = WK > 1 ? wave : 0;
     const int64_t m0 = (int64_t)blockIdx.x * BM;
@@ -169,19 +170,17 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 #pragma unroll
         for (int j = 0; j < NJ; ++j) q[j] = (g.ws + __builtin_amdgcn_readfirstlane(((first + j < g.t32 ? first + j : g.t32 - 1) * g.S4 + t) * 64))[lane];
     };
-    f32x16_t acc[MI][NJ];
-    const unsigned char* arow = smem + (wm * MI * 32 + (lane & 31)) * g.pitch + (lane >> 5) * 16;
-    const unsigned char* srow = smem + g.sc_ofs + (wm * MI * 32 + (lane & 31)) * g.spitch + (lane >> 5) * 4;
-    // steps s (with byte U of the scale words) and s + 1
+    f32x16_t acc[NJ];
+    const unsigned char* arow = smem + (wm * RT * 32 + (lane & 31)) * g.pitch + (lane >> 5) * 16;
+    const unsigned char* srow = smem + g.sc_ofs + (wm * RT * 32 + (lane & 31)) * g.spitch + (lane >> 5) * 4;
+    // step s + u of row tile i (byte U of the scale words)
 #define MXL_STEP(B, u, U)                                                                                                               \
     if (s + u < s1) {                                                                                                                   \
-        _Pragma("unroll") for (int i = 0; i < MI; ++i) {                                                                                \
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(arow + i * 32 * g.pitch + (s + u - s0) * 32);                           \
-            const i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};                                                    \
-            _Pragma("unroll") for (int j = 0; j < NJ; ++j) {                                                                            \
-                const i32x8_t bv = {(int)B.f[u][j].x, (int)B.f[u][j].y, (int)B.f[u][j].z, (int)B.f[u][j].w, 0, 0, 0, 0};                \
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[i][j], 4, 4, U, (int)sa[i], U, (int)sb[j]);     \
-            }                                                                                                                           \
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(arow + i * 32 * g.pitch + (s + u - s0) * 32);                               \
+        const i32x8_t av = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};                                                        \
+        _Pragma("unroll") for (int j = 0; j < NJ; ++j) {                                                                                \
+            const i32x8_t bv = {(int)B.f[u][j].x, (int)B.f[u][j].y, (int)B.f[u][j].z, (int)B.f[u][j].w, 0, 0, 0, 0};                    \
+            acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, acc[j], 4, 4, U, (int)sa, U, (int)sb[j]);                  \
         }                                                                                                                               \
     }
     // eight finished columns of a row; rv: the residual input there (zeros: none)
@@ -206,6 +205,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
     uint32_t sb[NJ];
     if (resident) {
         loadb(B0, 0, 4 * wk);                                     // in flight while the rows are quantised
+        if (RT > 1) loadb(B1, 0, 2);
         loads(sb, 0, wk);
         stage(0, g.S);
         __syncthreads();
@@ -215,110 +215,124 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
         const int n0 = ((blockIdx.y * g.per_wg + it) * WN + wn) * EPN;
         if (resident && WK == 1 && n0 >= g.N) break;              // (no barrier below in that form)
         const int nl = WK > 1 ? tid % LPR : lane % LPR, nc = n0 + nl * 8, left = g.N - nc;
-        // the residual rows are asked for before the products: their latency is the longest here
-        MxRaw8<T> rv[WK == 1 ? MI * 2 * NQ : 1];
-        if (WK == 1 && g.res) {
+#pragma unroll 1
+        for (int i = 0; i < RT; ++i) {
+            const int64_t mt = m0 + (wm * RT + i) * 32;
+            // the residual rows are asked for before the products: their latency is the longest here
+            MxRaw8<T> rv[WK == 1 ? 2 * NQ : 1];
+            if (WK == 1 && g.res) {
 #pragma unroll
-            for (int q = 0; q < MI * 2 * NQ; ++q) {
-                const int64_t m = m0 + wm * MI * 32 + q * RPI + lane / LPR;
-                rv[q].template load<FULLN>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M, g.N);
+                for (int q = 0; q < 2 * NQ; ++q) {
+                    const int64_t m = mt + q * RPI + lane / LPR;
+                    rv[q].template load<FULLN>(reinterpret_cast<const T*>(g.res), m * g.N + nc, left, m < g.M, g.N);
+                }
+                MX_LOADS_OUT();
             }
-            MX_LOADS_OUT();
-        }
-#pragma unroll
-        for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        for (int s0 = 0; s0 < g.S; s0 += resident ? g.S : g.chunk) {
-            const int s1 = resident || s0 + g.chunk > g.S ? g.S : s0 + g.chunk;
-            int s = s0 + 4 * wk;
-            if (!resident) {
-                __syncthreads();
-                loadb(B0, it, s);
-                loads(sb, it, s >> 2);
-                stage(s0, s1);
-                __syncthreads();
-            }
-            for (; s < s1; s += 4 * WK) {
-                uint32_t sa[MI], sn[NJ];
-#pragma unroll
-                for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(srow + i * 32 * g.spitch + ((s - s0) >> 2) * 8);
-                loadb(B1, it, s + 2);
-                loads(sn, it, (s >> 2) + WK);
+                for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
+            if (RT > 1) {
+                constexpr int s0 = 0;
+                const int s1 = g.S;
+                const uint32_t sa = *reinterpret_cast<const uint32_t*>(srow + i * 32 * g.spitch);
+                int s = 0;
                 MXL_STEP(B0, 0, 0) MXL_STEP(B0, 1, 1)
-                loadb(B0, it, s + 4 * WK);
-                s += 2;
+                s = 2;
                 MXL_STEP(B1, 0, 2) MXL_STEP(B1, 1, 3)
-                s -= 2;
+                if (i == RT - 1 && it + 1 < g.per_wg) {
+                    loadb(B0, it + 1, 0);
+                    loadb(B1, it + 1, 2);
+                    loads(sb, it + 1, 0);
+                }
+            } else {
+                for (int s0 = 0; s0 < g.S; s0 += resident ? g.S : g.chunk) {
+                    const int s1 = resident || s0 + g.chunk > g.S ? g.S : s0 + g.chunk;
+                    int s = s0 + 4 * wk;
+                    if (!resident) {
+                        __syncthreads();
+                        loadb(B0, it, s);
+                        loads(sb, it, s >> 2);
+                        stage(s0, s1);
+                        __syncthreads();
+                    }
+                    for (; s < s1; s += 4 * WK) {
+                        const uint32_t sa = *reinterpret_cast<const uint32_t*>(srow + ((s - s0) >> 2) * 8);
+                        uint32_t sn[NJ];
+                        loadb(B1, it, s + 2);
+                        loads(sn, it, (s >> 2) + WK);
+                        MXL_STEP(B0, 0, 0) MXL_STEP(B0, 1, 1)
+                        loadb(B0, it, s + 4 * WK);
+                        s += 2;
+                        MXL_STEP(B1, 0, 2) MXL_STEP(B1, 1, 3)
+                        s -= 2;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) sb[j] = sn[j];
+                        for (int j = 0; j < NJ; ++j) sb[j] = sn[j];
+                    }
+                }
+                if (resident && it + 1 < g.per_wg) {
+                    loadb(B0, it + 1, 4 * wk);
+                    loads(sb, it + 1, wk);
+                }
             }
-        }
-        if (resident && it + 1 < g.per_wg) {
-            loadb(B0, it + 1, 4 * wk);
-            loads(sb, it + 1, wk);
-        }
-        float bs[8];
+            float bs[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bs[e] = 0.f;
-        if (g.bias) {
-            MxRaw8<float> b;
-            b.template load<FULLN>(g.bias, nc, left, true, g.N);
-            b.template fix<FULLN>();
-            b.get(bs);
-        }
-        if (WK == 1) {
-            // 16 rows at a time through the wave's own slice of LDS, then eight columns a lane
-            float* ep = reinterpret_cast<float*>(smem + g.ep_ofs) + wave * 16 * EPP;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int e = 0; e < 8; ++e) bs[e] = 0.f;
+            if (g.bias) {
+                MxRaw8<float> b;
+                b.template load<FULLN>(g.bias, nc, left, true, g.N);
+                b.template fix<FULLN>();
+                b.get(bs);
+            }
+            if (WK == 1) {
+                // 16 rows at a time through the wave's own slice of LDS, then eight columns a lane
+                float* ep = reinterpret_cast<float*>(smem + g.ep_ofs) + wave * 16 * EPP;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) ep[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[i][j][8 * h + e];
+                        for (int e = 0; e < 8; ++e) ep[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[j][8 * h + e];
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
                     for (int q = 0; q < NQ; ++q) {
                         const int r = q * RPI + lane / LPR;
                         const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + r * EPP + nl * 8), hi = *reinterpret_cast<const f32x4_t*>(ep + r * EPP + nl * 8 + 4);
                         float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                        finish(v, rv[(i * 2 + h) * NQ + q], m0 + (wm * MI + i) * 32 + h * 16 + r, nc, left, bs);
+                        finish(v, rv[h * NQ + q], mt + h * 16 + r, nc, left, bs);
                     }
                 }
-        } else {
-            float* ep = reinterpret_cast<float*>(smem + g.ep_ofs);
-            __syncthreads();
+            } else {
+                float* ep = reinterpret_cast<float*>(smem + g.ep_ofs);
+                __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ep[(wk * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[0][j][e];
-            __syncthreads();
-            for (int r = tid / LPR; r < rows; r += 256 / LPR) {
-                if (g.res) rv[0].template load<FULLN>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true, g.N);
-                float v[8];
+                    for (int e = 0; e < 16; ++e) ep[(wk * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[j][e];
+                __syncthreads();
+                for (int r = tid / LPR; r < rows; r += 256 / LPR) {
+                    if (g.res) rv[0].template load<FULLN>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true, g.N);
+                    float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;
+                    for (int e = 0; e < 8; ++e) v[e] = 0.f;
 #pragma unroll
-                for (int k = 0; k < WK; ++k) {
-                    const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8), hi = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8 + 4);
+                    for (int k = 0; k < WK; ++k) {
+                        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8), hi = *reinterpret_cast<const f32x4_t*>(ep + (k * 32 + r) * EPP + nl * 8 + 4);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
+                        for (int e = 0; e < 4; ++e) { v[e] += lo[e]; v[4 + e] += hi[e]; }
+                    }
+                    finish(v, rv[0], m0 + r, nc, left, bs);
                 }
-                finish(v, rv[0], m0 + r, nc, left, bs);
             }
         }
     }
 #undef MXL_STEP
 }
 
-template <typename T, int MI, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN>
+template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN>
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
-    constexpr int BM = 32 * MI * WM, EPP = 32 * NJ + 4;
+    constexpr int BM = 32 * RT * WM, EPP = 32 * NJ + 4;
     const int ep = (WK > 1 ? 4 * 32 : 4 * 16) * EPP * 4;
     // LDS holds all channels of the rows where they fit, else a chunk at a time
     int chunk = g.S;
@@ -345,26 +359,29 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     int dev = 0;
     CN_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
-        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        if constexpr (RT == 1)
+            CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (dev < 64) attr[dev] = true;
     }
     const dim3 grid((unsigned)mt, (unsigned)split);
-    if (chunk >= g.S) mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, 256, smem, st>>>(g);
-    else mx_linear_kernel<T, MI, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, 256, smem, st>>>(g);
+    if (RT > 1 || chunk >= g.S) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, 256, smem, st>>>(g);
+    else if constexpr (RT == 1) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, 256, smem, st>>>(g);
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
 }
 // Which waves do what, us (bf16, M x K x N):
-//   K split over the waves, 32 x 32 a workgroup | columns over the waves, 32 x 256: 1x2048x512 4.5 | -, 64x1440x64 8.8 | 10.3, 512x2048x512
-//     10.9 | 13.0, 2048x64x256 5.1 | 5.5, 20000x1440x8 15.4 | 17.5; the other way 512x512x2048 9.3 | 6.6, 8192x512x64 6.9 | 6.4, 8192x1024x256 15.2 | 10.0
-//   rows over the waves, 128 x 64 | 64 x 128 | 32 x 256: 65536x64x64 7.4 | 8.7 | 11.4, 65536x256x128 16.4 | 13.0 | 14.5, 65536x64x256
-//     13.4 | 12.9 | 14.7, 65536x512x64 17.5 | 17.4 | 16.4, 65536x1024x256 111 | 53 | 45, 65536x256x1024 93 | 71 | 68
+//   K split over the waves, 32 x 32 a workgroup | columns over the waves, 32 x 256: 64x1440x64 8.8 | 10.3, 512x2048x512 10.9 | 13.0,
+//     2048x64x256 5.1 | 5.5, 20000x1440x8 15.4 | 17.5; the other way 512x512x2048 9.3 | 6.6, 8192x512x64 6.9 | 6.4, 8192x1024x256 15.2 | 10.0
+//   rows over the waves, 128 x 64 | 64 x 128 | 32 x 256: 65536x64x64 7.4 | 8.7 | 11.4, 65536x256x128 16.4 | 13.3 | 14.7, 65536x512x64
+//     17.5 | 17.4 | 16.4, 65536x1024x256 111 | 53 | 44
+//   32 x 256 | two row tiles, 64 x 256: 65536x256x1024 with its residual 69 | 63, 262144x64x256 52 | 41, 32768x256x512 14.4 | 15.7
 template <typename T, bool FULLK, bool FULLN>
 static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
     if (g.N <= 32 || (g.M + 31) / 32 * cdiv(g.N, 32) <= 512) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
     if (g.N <= 64 && g.K <= 256) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
-    if ((g.N <= 128 && g.K <= 256) || g.K <= 64) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
+    if (g.N <= 128 && g.K <= 256) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
+    if (g.K <= 256 && g.M >= 49152) return mxl_launch<T, 2, 2, 1, 4, 1, FULLK, FULLN>(g, st);
     return mxl_launch<T, 1, 2, 1, 4, 1, FULLK, FULLN>(g, st);
 }
 

@@ -190,7 +190,7 @@ def test_checkpoint_signs(dt, rows, C):
 
 # ------------------------------------------------------------------------------------------------ product
 LINEAR = [(1, 1, 1), (1, 32, 32), (1, 2048, 512), (2, 64, 80), (31, 16, 64), (33, 77, 5), (64, 100, 200), (65, 513, 130), (129, 208, 65),
-          (200, 1100, 300), (130, 4096, 260), (67, 4500, 70), (300, 2100, 100), (5, 9000, 40), (128, 512, 1024), (1000, 64, 64), (257, 256, 2048), (20000, 72, 4), (40, 2056, 3)]
+          (200, 1100, 300), (130, 4096, 260), (67, 4500, 70), (300, 2100, 100), (5, 9000, 40), (128, 512, 1024), (1000, 64, 64), (257, 256, 2048), (20000, 72, 4), (40, 2056, 3), (50001, 200, 264), (49153, 33, 130)]
 
 
 @pytest.mark.parametrize("dt", [BF, F32])
