@@ -417,3 +417,43 @@ def test_captured_and_replayed():
         assert all(torch.equal(p, q) for p, q in zip(eager, wants[rep % 2]))
         for o, w in zip(outs, wants):
             assert all(torch.equal(p, q) for p, q in zip(o, w)), rep
+
+
+def test_two_threads():
+    """two host threads, a stream each, call everything at once"""
+    import threading
+    ins = [_inputs(1), _inputs(30)]
+    wants = [_pass(*a) for a in ins]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    got = _pass(*ins[k])
+                    s.synchronize()
+                    assert all(torch.equal(p, q) for p, q in zip(got, wants[k]))
+        except BaseException as e:      # noqa: BLE001 - reported by the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_a_device_that_is_not_the_current_one():
+    a = _inputs(1)
+    want = _pass(*a)
+    with torch.cuda.device(0):
+        b = [t.to("cuda:1") if isinstance(t, torch.Tensor) else mx().MXWeight(t.packed.to("cuda:1"), t.out_features, t.in_features) for t in a]
+        torch.cuda.synchronize(1)
+        got = _pass(*b)
+        torch.cuda.synchronize(1)
+    assert all(t.device.index == 1 for t in got)
+    assert all(torch.equal(p, q.to(p.device)) for p, q in zip(want, got))
