@@ -40,8 +40,8 @@ class MXTensor:
         n = self._n * ((33 if fmt == "e4m3" else 17) + (4 if signs else 0))
         if buffer is None:
             buffer = torch.empty(n, dtype=torch.uint8, device=device)
-        elif buffer.numel() != n:
-            raise ValueError(f"MXTensor: a buffer of {n} bytes is needed, got {buffer.numel()}")
+        elif buffer.numel() != n or buffer.dtype != torch.uint8 or not buffer.is_contiguous():
+            raise ValueError(f"MXTensor: a contiguous uint8 buffer of {n} bytes is needed, got {tuple(buffer.shape)} {buffer.dtype}")
         self.buffer = buffer
 
     @property
@@ -91,10 +91,13 @@ class MXTensor:
 
 class MXWeight:
     """e2m1 weights of a linear layer / 1x1 convolution in the product's own order (`pack_weight`)."""
-    __slots__ = ("packed", "out_features", "in_features")
+    __slots__ = ("packed", "out_features", "in_features", "_n")
 
     def __init__(self, packed, out_features, in_features):
+        if packed.dtype != torch.uint8 or not packed.is_contiguous():
+            raise ValueError("MXWeight: packed must be contiguous uint8")
         self.packed, self.out_features, self.in_features = packed, out_features, in_features
+        self._n = _hip.query("cn_mx_weight_bytes", out_features, in_features)
 
     def __repr__(self):
         return f"MXWeight({self.out_features}, {self.in_features})"
@@ -162,6 +165,8 @@ def dequantize(q, dtype=None):
     dtype = dtype or q.dtype
     if dtype not in _DTYPES:
         raise TypeError(f"mx.dequantize: unsupported dtype {dtype} (bfloat16 or float32)")
+    if not q.buffer.is_cuda:
+        raise RuntimeError("mx.dequantize: tensor is not on the GPU (no CPU path exists)")
     out = torch.empty(q.shape, dtype=dtype, device=q.buffer.device)
     codes, scales, _ = q._pointers()
     launch("cn_mx_dequantize", out.get_device(), codes, scales, out.data_ptr(), q.rows, q.shape[-1], FORMATS[q.fmt], _DTYPES[dtype])
@@ -198,6 +203,8 @@ def linear(x, weight, bias=None, residual=None, relu=False):
         raise ValueError(f"mx.linear: x has {x.shape[-1]} channels, weight expects {K}")
     if weight.packed.device != dev:
         raise ValueError(f"mx.linear: weight on {weight.packed.device}, x on {dev}")
+    if weight.packed.numel() != weight._n:
+        raise ValueError(f"mx.linear: packed weights of {weight._n} bytes are needed, got {weight.packed.numel()}")
     lead = x.shape[:-1]
     shape = (*lead, N)
     if bias is not None:
@@ -219,7 +226,8 @@ def _checkpoint_of(ck, dy, what):
 
 def linear_wgrad(dy, ck, bias=False, into=None, bias_into=None):
     """Gradients of a linear layer / 1x1 convolution whose input was kept as `ck`: -> (dw fp32 [N, K], db fp32 [N] | None) for
-    dy [..., N].  into / bias_into: contiguous fp32 tensors (of N * K / N values) the gradients are added to instead."""
+    dy [..., N].  into / bias_into: contiguous fp32 tensors (of N * K / N values) the gradients are added to instead.  N and K of which
+    more than 65535 output tiles (of 64 x 64 up to 128 x 128 values) would be needed are refused."""
     dy, dt = _tensor(dy, "mx.linear_wgrad")
     _checkpoint_of(ck, dy, "mx.linear_wgrad")
     if dy.shape[:-1] != ck.shape[:-1]:

@@ -457,3 +457,14 @@ def test_on_a_device_that_is_not_the_current_one():
         torch.cuda.synchronize(1)
     assert all(t.device.index == 1 for t in got)
     assert all(torch.equal(p, q.to(p.device)) for p, q in zip(want, got))
+
+
+def test_packed_weights_of_another_size_are_refused():
+    w = mx().pack_weight(torch.randn(40, 70, device="cuda"))
+    x = torch.randn(3, 70, device="cuda")
+    again = mx().MXWeight(w.packed.clone(), 40, 70)
+    assert torch.equal(mx().linear(x, w), mx().linear(x, again))
+    with pytest.raises(ValueError, match="packed weights"):
+        mx().linear(x, mx().MXWeight(w.packed[:-256], 40, 70))
+    with pytest.raises(ValueError, match="packed weights"):
+        mx().linear(torch.randn(3, 200, device="cuda"), mx().MXWeight(w.packed, 40, 200))

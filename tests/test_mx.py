@@ -108,6 +108,22 @@ def test_python_refusals(lib):
         m.linear(x.requires_grad_(), m.MXWeight(torch.zeros(1, dtype=torch.uint8), 8, 32))
 
 
+def test_buffers_of_the_wrong_kind_are_refused(lib):
+    """a buffer that came back from a file or another device is checked before a kernel could read beyond it"""
+    m, shape = mx(), torch.Size((4, 40))
+    meta = (shape, torch.float32, "e4m3", False)
+    n = 4 * 2 * 33
+    assert m.MXTensor.of(torch.zeros(n, dtype=torch.uint8), meta).nbytes() == n
+    for bad in (torch.zeros(n - 1, dtype=torch.uint8), torch.zeros(n), torch.zeros(1, dtype=torch.uint8).expand(n), torch.zeros(2 * n, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="uint8 buffer"):
+            m.MXTensor.of(bad, meta)
+    with pytest.raises(RuntimeError, match="not on the GPU"):
+        m.dequantize(m.MXTensor.of(torch.zeros(n, dtype=torch.uint8), meta))
+    for bad in (torch.zeros(1 * 1024 + 256), torch.zeros(1, dtype=torch.uint8).expand(1280)):
+        with pytest.raises(ValueError, match="contiguous uint8"):
+            m.MXWeight(bad, 8, 32)
+
+
 # ---- the oracle -----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt,largest,tie", [("e2m1", 6.0, 7.0), ("e4m3", 448.0, 464.0)])
 def test_oracle_scale_rule(fmt, largest, tie):
