@@ -9,7 +9,7 @@
 //   * the bilinear geometry of all 9 taps of the tile (h0, w0, lh, lw, mask), computed once per tile from offsets that were
 //     prefetched during the previous tile;
 //   * a double-buffered A tile [128 px][64 ch]: 4 lanes per pixel blend 16 channels each from four 32-byte LDS corner reads
-//     (fp32 weights, v_pk_fma_f32), while the matrix cores multiply the previous tap's tile with its weight slice (3-deep
+//     (fp32 weights), while the matrix cores multiply the previous tap's tile with its weight slice (3-deep
 //     register ring, L2-resident).
 // Corners outside the halo (offsets beyond about +-2 px) fall back to masked global loads.  The output tile leaves through LDS
 // as 16-byte vectors with bias / ReLU applied in fp32.

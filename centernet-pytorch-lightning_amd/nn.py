@@ -37,6 +37,12 @@ class Conv2d(nn.Module):
             self.register_parameter("bias", None)
         self._cache = {}
 
+    def __getstate__(self):
+        """copies and pickles pack their 4-bit weights again: a copied parameter starts at version 0"""
+        state = self.__dict__.copy()
+        state.pop("_mx_cache", None)
+        return state
+
     def extra_repr(self):
         co, ci, k, _ = self.weight.shape
         return f"{ci}, {co}, kernel_size={k}, stride={self.stride}, padding={self.padding}, bias={self.bias is not None}"
@@ -88,12 +94,12 @@ class Conv2d(nn.Module):
         return ops._igemm(x, c["wp"], c["b"], residual, Co, KH, KW, self.stride, self.padding, False, relu, OH, OW, out_dtype)
 
     def _mx_weight(self, x, scale, shift):
-        """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels; kept per
-        weight version like `infer_key`'s"""
-        key = (x.shape[-1], x.device, self.weight._version, None if self.bias is None else self.bias._version, ops.WeightsEpoch.value,
-               None if scale is None else (scale.data_ptr(), scale._version))
+        """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels; kept while
+        the tensors they were made from are these, unchanged (versions; the entry holds the tensors, so no other takes their place)"""
+        made = (self.weight, self.bias, scale, shift)
+        key = (x.shape[-1], x.device, ops.WeightsEpoch.value, *(None if t is None else t._version for t in made))
         hit = self.__dict__.get("_mx_cache")
-        if hit is None or hit[0] != key:
+        if hit is None or hit[0] != key or any(a is not b for a, b in zip(hit[3], made)):
             Co, Ci = self.weight.shape[:2]
             with torch.no_grad():
                 w = torch.zeros(ops.rup(Co, 16), x.shape[-1], dtype=torch.float32, device=x.device)
@@ -103,7 +109,7 @@ class Conv2d(nn.Module):
                     b[:Co] = self.bias if scale is None else self.bias * scale
                 if shift is not None:
                     b[:Co] += shift
-            hit = (key, mx.pack_weight(w), b)
+            hit = (key, mx.pack_weight(w), b, made)
             if not torch.cuda.is_current_stream_capturing():       # (what a capture packs exists only once the graph has run)
                 self._mx_cache = hit
         return hit[1], hit[2]

@@ -273,6 +273,34 @@ def test_root_and_head_inference_in_4_bits():
         within(y.permute(0, 2, 3, 1).reshape(-1, 20), want, half_step(BF) * np.abs(want) + 72 * U * m, "head")
 
 
+def test_weights_of_a_copy_or_another_parameter_are_packed_anew():
+    """a copied parameter starts at version 0, and one put in another's place may have its version: what was packed for the first must not
+    answer for the second"""
+    n = hnn()
+    conv = n.Conv2d(64, 32, 1).to(DEV)
+    n.use_mxfp4(conv)
+    x = img((1, 4, 4, 64), 1, F32)
+    sds = [{"weight": rnd((32, 64, 1, 1), 5 + i, F32)} for i in range(3)]
+
+    def fresh(sd):
+        c = n.Conv2d(64, 32, 1).to(DEV)
+        n.use_mxfp4(c)
+        c.load_state_dict(sd)
+        return c(x)
+
+    with torch.no_grad():
+        wants = [fresh(sd) for sd in sds]
+        conv.load_state_dict(sds[0], assign=True)
+        conv.weight.mul_(1)                                        # version 1
+        assert conv.weight._version == 1 and torch.equal(conv(x), wants[0])
+        other = copy.deepcopy(conv)
+        other.load_state_dict(sds[1])                              # version 1 again
+        assert other.weight._version == 1 and other.mx4 and torch.equal(other(x), wants[1])
+        for i in (2, 1, 0):
+            conv.load_state_dict({k: v.clone() for k, v in sds[i].items()}, assign=True)
+            assert conv.weight._version == 0 and torch.equal(conv(x), wants[i])
+
+
 def test_inference_captured_before_any_eager_call():
     """weights packed during a capture are not kept for eager calls (they hold nothing until the graph has run)"""
     n = hnn()

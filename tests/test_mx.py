@@ -124,6 +124,17 @@ def test_buffers_of_the_wrong_kind_are_refused(lib):
             m.MXWeight(bad, 8, 32)
 
 
+def test_copies_of_a_layer_leave_packed_weights_behind():
+    import copy
+    import pickle
+    from centernet_amd import nn as hnn
+    conv = hnn.Conv2d(32, 16, 1)
+    conv._mx_cache = ("key", "weights", "bias", ())
+    for c in (copy.deepcopy(conv), copy.copy(conv), pickle.loads(pickle.dumps(conv))):
+        assert "_mx_cache" not in c.__dict__ and torch.equal(c.weight, conv.weight)
+    assert conv._mx_cache[0] == "key"
+
+
 # ---- the oracle -----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("fmt,largest,tie", [("e2m1", 6.0, 7.0), ("e4m3", 448.0, 464.0)])
 def test_oracle_scale_rule(fmt, largest, tie):
