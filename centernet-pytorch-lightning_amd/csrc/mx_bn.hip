@@ -7,9 +7,9 @@
 // x8 is what the e4m3 codes stand for.  The sums need every row before the first dx, so dy and the codes are read twice: 2 x 3.16
 // bytes per bf16 element in, 2 (4 with a residual input) out.  A thread owns eight channels and walks rows, so the sums and the
 // coefficients stay in registers; partial sums are joined in a fixed order (results do not depend on the schedule).
+// Bound by memory: 262144 x 256 bf16, with ReLU, sums 37 us (211 MB, 5.7 TB/s), finish 5, dx 74 (345 MB, 4.7 TB/s: reads and writes mixed);
+// 512 x 512 7.1 us in one launch.
 #include "mx_common.h"
-
-#define MXBN_MAX_GROUPS 1024
 
 struct MxBnGeom {
     const void* dy;
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void mx_bn_sums_kernel(const MxBnGeom g, const
 }
 
 // Four channels a workgroup, a thread per partial row: totals, parameter gradients, and the coefficients a, b, c of dx.  The partial sums
-// were written from all over the card: few workgroups with long chains of such reads cost 19 us for 1024 x 256 channels, this 7 us.
+// were written from all over the card: few workgroups with long chains of such reads cost 19 us for 1024 rows of 256 channels, this 7 us.
 __global__ __launch_bounds__(256) void mx_bn_finish_kernel(const float* __restrict__ part, int groups, int C, int ld, float inv_rows,
                                                            const float* __restrict__ gamma, const float* __restrict__ invstd,
                                                            float* __restrict__ coef, float* __restrict__ dgamma, float* __restrict__ dbeta,
@@ -309,8 +309,9 @@ __global__ __launch_bounds__(NT) void mx_bn_small_kernel(const MxBnGeom g, const
     }
 }
 
-// rows of four chunks that a workgroup holds.  us, one launch | two or three: 128x512 5.3 | 10, 512x512 7.2 | 11, 700x512 8.3 | 11.6; eight rows
-// a thread for 2048 rows: 1471x30 16 | 10.2
+// rows of four chunks that a workgroup holds.  us, one launch | two or three: 128x512 5.3 | 10, 512x512 7.1 | 11, 700x512 8.3 | 11.6; eight rows
+// a thread for 2048 rows: 1471x30 16 | 10.2.  Threads and rows of one: 128x512 in 256 threads 5.3, in 1024 5.6; 512x2048 with two rows 7.6,
+// with four 7.8
 #define MXBN_SMALL 1024
 
 static int mxbn_lg(int C) {
@@ -319,14 +320,17 @@ static int mxbn_lg(int C) {
     while (lg < 5 && (1 << lg) < chunks) ++lg;
     return lg;
 }
-#define MXBN_JOIN 32           // row groups up to which the apply pass adds the partial sums up itself
-// row groups of the sums pass: ~1024 workgroups in all, at least four rows for a thread
+// row groups up to which the apply pass adds the partial sums up itself: a launch less for the host (3 us there), and little more on the
+// device (4515x28 11.7 us, 10.9 with a finish pass; up to 128 groups 4096x256 would take 39 instead of 11.4)
+#define MXBN_JOIN 32
+// row groups of the sums pass: ~512 workgroups in all, at least four rows for a thread.  us, 256 | 512 | 1024 | 2048 workgroups: 262144x256
+// 118 | 106 | 111 | 116, 1048576x64 118 | 106 | 108 | 112, 16384x512 21.3 | 21.6 | 23.7 | 23.7
 static int mxbn_groups(int64_t rows, int C) {
     const int lg = mxbn_lg(C), tiles = cdiv(cdiv(C, 8), 1 << lg);
     const int64_t most = (rows + 4 * (256 >> lg) - 1) / (4 * (256 >> lg));
-    int64_t g = 1024 / tiles;
+    int64_t g = 512 / tiles;
     g = g < most ? g : most;
-    return (int)(g < 1 ? 1 : (g > MXBN_MAX_GROUPS ? MXBN_MAX_GROUPS : g));
+    return (int)(g < 1 ? 1 : g);
 }
 
 extern "C" size_t cn_mx_bn_bwd_bytes(int64_t rows, int C, int dtype) {
@@ -387,9 +391,10 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
         mx_bn_finish_kernel<<<cdiv(C, 4), 256, 0, st>>>(part, groups, C, ld, t.inv_rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
         CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     }
-    // eight rows a thread (its coefficients are loaded once), fewer where that would leave compute units idle
+    // eight rows a thread (its coefficients are loaded once), fewer where that would leave less than two workgroups a compute unit (us, this
+    // rule | always two rows | always eight: 4515x28 11.7 | 12.0 | 14.7, 8192x256 13.2 | 13.2 | 14.1, 262144x256 110 | 113 | 110)
     int deep = 8;
-    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 1024) deep /= 2;
+    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
     g.per = (int64_t)deep * nrl;
     CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_bn_bwd: too many rows");
     const int ng = cdiv(rows, g.per);

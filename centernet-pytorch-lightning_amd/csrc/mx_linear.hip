@@ -5,6 +5,8 @@
 // What has to move is x in and y out; the codes of x never leave the workgroup.  A workgroup quantises its BM rows once into LDS and
 // keeps them there while it walks all its columns, so x is read from memory once whatever N is; the weights stream from L2 in
 // fragment order (1 KB contiguous per 32 columns x 64 channels).  K beyond what LDS holds is taken in chunks.
+// Bound by memory: 65536x256x1024 with its residual 57 us (302 MB, 5.3 TB/s, the rate of a copy), 65536x1024x256 41 us (168 MB, 4.1 TB/s:
+// reading x alone takes 28, quantising, products and stores overlap with it in part), 1x2048x512 4.4 us (latency of one row's K).
 #include "mx_common.h"
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
@@ -350,7 +352,9 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     const int64_t mt = (g.M + BM - 1) / BM;
     if (mt >= ((int64_t)1 << 31)) { cn_set_error("cn_mx_linear_fwd: too many rows"); return CN_EINVAL; }
     const int passes = cdiv(g.t32, NJ * WN);
-    // one workgroup walks all columns of its rows unless that leaves compute units idle
+    // one workgroup walks all columns of its rows unless that leaves less than four workgroups a compute unit.  us, never split | this rule |
+    // one pass a workgroup: 512x512x2048 16.8 | 6.5 | 6.8, 4096x512x2048 19.3 | 13.1 | 13.1, 16384x256x1024 14.8 | 14.9 | 17.1,
+    // 65536x256x1024 36.3 | 36.3 | 45.6 (no residual)
     int64_t split = mt >= 1024 ? 1 : (1024 + mt - 1) / mt;
     if (chunk < g.S || split > passes) split = passes;
     g.per_wg = cdiv(passes, split);

@@ -2,10 +2,13 @@
 //   dw[n][k] = sum_r dy[r][n] * x8[r][k],   db[n] = sum_r dy[r][n]
 //
 // The sum runs over rows, the slow axis of both operands.  Tiles are staged in their natural [row][channel] order — the e4m3 codes
-// become bf16 on the way (exact: four significant bits times a power of two) — and the transposing LDS read hands every lane eight
+// become bf16 on the way (exact: four significant bits times a power of two; what is below 2^-126 becomes zero) — and the transposing LDS read hands every lane eight
 // rows of its channel (rows padded by 64 B: the four rows of a read hit disjoint banks).  A 32-bit dy is split into three bf16 terms
 // (8 + 8 + 8 significant bits: nothing is lost) that share the x8 fragment.
 // Row ranges are split over workgroups; their partial sums go to the workspace and are added in a fixed order.
+// Measured: 262144x256x128 bf16 35 us + 6.5 us for the join (136 MB in: 3.9 TB/s; with the wide tiles dy and the codes are read twice and
+// once), 16384x512x2048 55 us = 0.62 PFLOP/s, where the LDS reads of a tile (768 cycles) take longer than its products (512); 1024x2048x512
+// 12.5 us, 16 row tiles in one workgroup a compute unit: latency.  32 bits: three products, 0.42 - 0.7 PFLOP/s.
 #include "mx_common.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -76,7 +79,9 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     constexpr int YV = BR * TN / 8 / 256, XV = BR * TK / 16 / 256;
     constexpr int YC = TN / 8, XC = TK / 16;
     constexpr int MI = TN / 64, NJ = TK / 64;                     // 2 x 2 waves of 32 x 32 tiles
-    constexpr int DEEP = TN * TK == 64 * 64 ? 2 : 1;              // tiles in flight: the wide tiles have no registers for a second
+    // tiles in flight.  The wide tiles have no registers for a second; in the narrow ones it pays for 16 bits (quantising and gradient of
+    // 1024x2048x512, one | two: 18.8 | 17.4 us), not for 32 (5883x208x80 15.5 | 16.4)
+    constexpr int DEEP = sizeof(T) == 2 && TN * TK == 64 * 64 ? 2 : 1;
     constexpr int PLANE = BR * YP;
     __shared__ __attribute__((aligned(16))) bf16_t lds[NP * PLANE + BR * XP];
     bf16_t* const ly = lds;
@@ -342,8 +347,9 @@ extern "C" int cn_mx_linear_wgrad(const void* dy, const void* codes, const void*
     if (join) {
         const int64_t n = (int64_t)N * K;
         const int nb = db ? N : 0;
-        // more groups where the splits are many and the outputs few; 16 / 64 / 1024 outputs a workgroup
-        if (p.splits >= 128 && n <= 4096) mx_wgrad_join_kernel<64><<<(unsigned)(cdiv(n, 16) + cdiv(nb, 16)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
+        // more groups where the splits are many and the outputs few; 16 / 64 / 1024 outputs a workgroup.  us, 64 | 16 | 1 groups: 15993x22x51
+        // 8.8 | 10.9 | 28, 65536x64x64 16.1 | 13.6 | 34, 65536x256x64 18.1 | 15.3 | 19.9; 8192x512x512 (few splits) 29.8 | 22.4 | 22.2
+        if (p.splits >= 64 && n <= 2048) mx_wgrad_join_kernel<64><<<(unsigned)(cdiv(n, 16) + cdiv(nb, 16)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         else if (p.splits >= 16) mx_wgrad_join_kernel<16><<<(unsigned)(cdiv(n, 64) + cdiv(nb, 64)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         else mx_wgrad_join_kernel<1><<<(unsigned)(cdiv(n, 1024) + cdiv(nb, 1024)), 256, 0, st>>>(g.dw, dw, n, p.splits, g.db, db, nb, accumulate);
         CN_LAUNCH_CHECK("cn_mx_linear_wgrad");
