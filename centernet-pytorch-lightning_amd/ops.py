@@ -765,9 +765,9 @@ def _input_checkpoint(x):
     return cell.ck[1]
 
 
-def _shape_only(ck):
-    """a tensor with the checkpointed input's shape and type and no memory, for code that reads nothing else of it"""
-    return torch.empty((1,) * len(ck.shape), dtype=ck.dtype, device=ck.device).expand(ck.shape)
+def _shape_only(t):
+    """a tensor with t's (or a checkpoint's) shape and type and no memory, for code that reads nothing else of it"""
+    return torch.empty((1,) * len(t.shape), dtype=t.dtype, device=t.device).expand(t.shape)
 
 
 def _ckpt_wgrad(dy, ck, weight, bias, order):
@@ -795,11 +795,12 @@ class Conv2dCkptFn(Function):
         Co, Ci, KH, KW = weight.shape
         N, H, W, Cx = x.shape
         assert Cx == rup(Ci, 16), f"conv input has {Cx} channels, weight expects {Ci}"
-        ck = _input_checkpoint(x)
+        ck = _input_checkpoint(x) if any(ctx.needs_input_grad[1:3]) else None          # (a frozen layer keeps nothing)
         y = _igemm(x, pack_weight(weight, 1, x.dtype), bias, None, Co, KH, KW, stride, pad, False, False, conv_out(H, KH, stride, pad),
                    conv_out(W, KW, stride, pad), bn_stats=bn_stats)
-        ctx.save_for_backward(ck.buffer, weight)
-        ctx.ck_meta = ck.meta
+        ctx.save_for_backward(None if ck is None else ck.buffer, weight)
+        ctx.ck_meta = None if ck is None else ck.meta
+        ctx.like = _shape_only(x)
         ctx.cfg = (stride, pad)
         ctx.bias_ref = bias
         ctx.order = SideGrads.next_order()
@@ -809,21 +810,21 @@ class Conv2dCkptFn(Function):
     @staticmethod
     def backward(ctx, dy):
         buffer, weight = ctx.saved_tensors
-        ck = mx.MXTensor.of(buffer, ctx.ck_meta)
+        ck = None if buffer is None else mx.MXTensor.of(buffer, ctx.ck_meta)
         (stride, pad), bias = ctx.cfg, ctx.bias_ref
         Co, Ci, KH, KW = weight.shape
         need = ctx.needs_input_grad
         dy = dy.contiguous()
-        if (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
-            dw = db = None
-            if need[1]:
-                dw, db = _ckpt_wgrad(dy, ck, weight, bias, ctx.order)
-            dx = _conv2d_bwd(_shape_only(ck), weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order,
-                             (need[0], False, False))[0]
+        x, dw, db, rest = ctx.like, None, None, (need[0], False, False)
+        if not need[1]:
+            if need[2]:                                # a frozen weight under a bias that is not
+                db = _wgrad_param(mx.dequantize(ck), dy, Co, Ci, KH, KW, stride, pad, want_bias=True)[1]
+        elif (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
+            dw, db = _ckpt_wgrad(dy, ck, weight, bias, ctx.order)
         else:
-            x = mx.dequantize(ck) if need[1] else _shape_only(ck)
-            dx, dw, db = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, need[:3])
-        return dx, dw, db, None, None, None
+            x, rest = mx.dequantize(ck), need[:3]
+        out = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, rest)
+        return (out[0], *(out[1:] if rest[1] else (dw, db)), None, None, None)
 
 
 def _cat_args(xs):

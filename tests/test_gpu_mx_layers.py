@@ -104,6 +104,33 @@ def test_conv_layer(dt, N, H, W, Ci, Co, k, s, p, bias):
         within(out["ck"][3], d.sum((0, 2, 3)).numpy(), terms * U * d.abs().sum((0, 2, 3)).numpy(), "db")
 
 
+@pytest.mark.parametrize("k,p", [(1, 0), (3, 1)])
+def test_conv_layer_with_frozen_parameters(k, p):
+    """a bias trains above a frozen weight; a layer that is frozen altogether passes the gradient on and keeps nothing"""
+    conv = hnn().Conv2d(32, 24, k, 1, p, bias=True).to(DEV)
+    hnn().use_checkpoints(conv)
+    conv.weight.requires_grad_(False)
+    x = img((2, 6, 6, 32), 1, F32).requires_grad_()
+    y = conv(x)
+    dy = img(tuple(y.shape), 2, F32, 1e-2)
+    dy[..., 24:] = 0
+    y.backward(dy)
+    dx = x.grad.clone()
+    d = f64(dy)[..., :24].reshape(-1, 24)
+    within(conv.bias.grad, d.sum(0), (3 * 72 + 16) * U * np.abs(d).sum(0), "db")
+    assert conv.weight.grad is None
+    want = torch.zeros(2, 32, 6, 6, dtype=torch.float64, requires_grad=True)
+    F.conv2d(want, conv.weight.detach().double().cpu(), None, 1, p).backward(torch.tensor(f64(dy)[..., :24]).permute(0, 3, 1, 2))
+    s = 24 * k * k * np.abs(f64(conv.weight)).max() * np.abs(d).max()
+    within(dx, want.grad.permute(0, 2, 3, 1).numpy(), np.full(dx.shape, (24 * k * k + 16) * U * s), "dx")
+    conv.bias.requires_grad_(False)
+    x.grad = None
+    y = conv(x)
+    assert y.grad_fn.saved_tensors[0] is None
+    y.backward(dy)
+    assert torch.equal(x.grad, dx)
+
+
 @pytest.mark.parametrize("dt", [BF, F32])
 def test_root_over_several_sources(dt):
     """conv1x1 over a concatenation that is never built, its sources shared with other layers and kept once"""
