@@ -516,6 +516,26 @@ extern "C" int cn_bn_train_fwd(const void* x, const void* residual, void* y, con
     return CN_OK;
 }
 
+extern "C" int cn_bn_train_stats(const void* x, const float* gamma, const float* beta, float* running_mean, float* running_var,
+                                 float* save_mean, float* save_invstd, float* save_scale_shift, int64_t npix, int C, float momentum,
+                                 float eps, int dtype, void* ws, size_t ws_bytes, void* stream) {
+    CN_CHECK_ARG(x && gamma && beta && save_mean && save_invstd && save_scale_shift && ws && npix > 0 && C > 0, "cn_bn_train_stats: bad args");
+    const int V = dtype == CN_F32 ? 4 : 8;
+    CN_CHECK_ARG(C % V == 0, "cn_bn_train_stats: C=%d must be a multiple of %d", C, V);
+    if (ws_bytes < cn_bn_workspace_bytes(npix, C)) { cn_set_error("cn_bn_train_stats: workspace too small"); return CN_EWORKSPACE; }
+    hipStream_t st = (hipStream_t)stream;
+    const BnLayout L = bn_layout(npix, C, V);
+    float* part = (float*)ws;
+    CN_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL((bn_partial_kernel<T, 0>), dim3(L.nblk, L.ycols), dim3(256), 0, st,
+                                                   (const T*)x, (const T*)nullptr, (const T*)nullptr, (const float*)nullptr,
+                                                   (const float*)nullptr, (const float*)nullptr, part, npix, C, L, 0, 0));
+    CN_LAUNCH_CHECK("cn_bn_train_stats(partial)");
+    hipLaunchKernelGGL(bn_finalize_fwd_kernel, dim3(cdiv(C, 4)), dim3(256), 0, st, part, L.nblk, C, npix, gamma, beta,
+                       running_mean, running_var, save_mean, save_invstd, save_scale_shift, (float*)nullptr, momentum, eps, (float*)nullptr);
+    CN_LAUNCH_CHECK("cn_bn_train_stats(finalize)");
+    return CN_OK;
+}
+
 // ---- statistics sink: the kernel that PRODUCES x accumulates sum x / sum x^2 in its epilogue (N1: conv + BN + ReLU in training) ----
 // cn_hooks.bn_part of a forward call (cn_conv2d_fwd_h, cn_conv1x1_cat_fwd_h, cn_dcn_fwd_h, cn_stem_conv_fwd_h): if the kernel the call
 // dispatches to has the hook, every workgroup adds the per-channel sums of the values it STORES (after rounding to the output dtype)

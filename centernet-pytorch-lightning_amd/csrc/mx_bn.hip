@@ -309,6 +309,65 @@ __global__ __launch_bounds__(NT) void mx_bn_small_kernel(const MxBnGeom g, const
     }
 }
 
+// a value as it is stored: what rounds to zero is not positive
+__device__ static inline float mx_stored(float v, const float*) { return v; }
+__device__ static inline float mx_stored(float v, const bf16_t*) { return bf2f(f2bf(v)); }
+
+// Forward: y = act(x scale + shift (+ residual)) and x's checkpoint in one pass (separately the checkpoint reads x and y again).  A thread
+// owns eight channels, filler included, and walks rows with its coefficients in registers; a quad of lanes is one block of 32.
+template <typename T, bool RES, bool RELU, bool FULL>
+__global__ __launch_bounds__(256) void mx_scale_shift_act_kernel(const MxBnGeom g, const T* __restrict__ x, const T* __restrict__ res,
+                                                                 const float* __restrict__ scale, const float* __restrict__ shift,
+                                                                 T* __restrict__ y, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                 uint8_t* __restrict__ signs) {
+    const int tid = threadIdx.x, tc = 1 << g.lg, cl = tid & (tc - 1), rl = tid >> g.lg, nrl = 256 >> g.lg;
+    const int c = blockIdx.y * tc + cl, left = g.C - c * 8;
+    if (c >= g.cpr) return;                                       // (whole quads: cpr and tc are multiples of four)
+    const int64_t r0 = (int64_t)blockIdx.x * g.per, r1 = r0 + g.per < g.rows ? r0 + g.per : g.rows;
+    float sc[8], sh[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { sc[j] = j < left ? scale[c * 8 + j] : 0.f; sh[j] = j < left ? shift[c * 8 + j] : 0.f; }
+    for (int64_t r = r0 + rl; r < r1; r += MXBN_U * nrl) {
+        MxRaw8<T> v[MXBN_U], w[RES ? MXBN_U : 1];
+#pragma unroll
+        for (int u = 0; u < MXBN_U; ++u) {
+            const int64_t at = (r + u * nrl) * g.C + c * 8;
+            v[u].template load<FULL>(x, at, left, r + u * nrl < r1, g.C);
+            if (RES) w[u].template load<FULL>(res, at, left, r + u * nrl < r1, g.C);
+        }
+        MX_LOADS_OUT();
+#pragma unroll
+        for (int u = 0; u < MXBN_U; ++u) {
+            const int64_t row = r + u * nrl;
+            if (row < r1) {                                       // (a quad's lanes have the same row)
+                v[u].template fix<FULL>();
+                const uint32_t b = mx_scale_byte<CN_MX_E4M3>(quad_max_u(v[u].absmax()));
+                float f[8], o[8];
+                v[u].get(f);
+                const int64_t i = row * g.cpr + c;
+                reinterpret_cast<uint2*>(codes)[i] = mx_codes_e4m3(f, b);
+                if ((c & 3) == 0) scales[i >> 2] = (uint8_t)b;
+                if (RES) {
+                    w[u].template fix<FULL>();
+                    w[u].get(o);
+                }
+                uint32_t m = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    f[j] = fmaf(f[j], sc[j], sh[j]);
+                    if (RES) f[j] += o[j];
+                    if (RELU) {
+                        f[j] = fmaxf(f[j], 0.f);
+                        m |= (mx_stored(f[j], (const T*)nullptr) > 0.f ? 1u : 0u) << j;
+                    }
+                }
+                mx_store8f<FULL>(y + row * g.C + c * 8, left, f);
+                if (RELU) signs[i] = (uint8_t)m;
+            }
+        }
+    }
+}
+
 // rows of four chunks that a workgroup holds.  us, one launch | two or three: 128x512 5.3 | 10, 512x512 7.1 | 11, 700x512 8.3 | 11.6; eight rows
 // a thread for 2048 rows: 1471x30 16 | 10.2.  Threads and rows of one: 128x512 in 256 threads 5.3, in 1024 5.6; 512x2048 with two rows 7.6,
 // with four 7.8
@@ -403,5 +462,36 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
 #undef MXBN_GO
 #undef MXBN_COMMA
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
+    return CN_OK;
+}
+
+extern "C" int cn_mx_scale_shift_act(const void* x, const void* residual, const float* scale, const float* shift, void* y, void* codes,
+                                     void* scales, void* signs, int64_t rows, int C, int relu, int dtype, void* stream) {
+    CN_CHECK_ARG(rows >= 0 && C >= 1 && C <= MX_MAX_C && rows <= ((int64_t)1 << 40) / C, "cn_mx_scale_shift_act: rows %lld, channels %d", (long long)rows, C);
+    CN_CHECK_ARG(dtype == CN_F32 || dtype == CN_BF16, "cn_mx_scale_shift_act: bad dtype %d", dtype);
+    CN_CHECK_ARG((signs != nullptr) == (relu != 0), "cn_mx_scale_shift_act: signs come with relu");
+    if (rows == 0) return CN_OK;
+    CN_CHECK_ARG(x && scale && shift && y && codes && scales, "cn_mx_scale_shift_act: null pointer");
+    CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_scale_shift_act: codes must be 16-byte aligned");
+    MxBnGeom g{nullptr, nullptr, nullptr, nullptr, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 2, 0};
+    while (g.lg < 5 && (1 << g.lg) < g.cpr) ++g.lg;
+    const int tiles = cdiv(g.cpr, 1 << g.lg), nrl = 256 >> g.lg;
+    int deep = 8;                                                 // (rows a thread: as in the backward pass)
+    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
+    g.per = (int64_t)deep * nrl;
+    CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_scale_shift_act: too many rows");
+    const dim3 grid(cdiv(rows, g.per), tiles);
+    hipStream_t st = (hipStream_t)stream;
+#define MXSS(RES, RELU, FULL)                                                                                                          \
+    mx_scale_shift_act_kernel<T, RES, RELU, FULL><<<grid, 256, 0, st>>>(g, (const T*)x, (const T*)residual, scale, shift, (T*)y,       \
+                                                                        (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)signs)
+#define MXSS_F(RES, RELU) do { if (C % 8 == 0) MXSS(RES, RELU, true); else MXSS(RES, RELU, false); } while (0)
+    CN_DISPATCH_DTYPE(dtype, T, {
+        if (residual) { if (relu) MXSS_F(true, true); else MXSS_F(true, false); }
+        else { if (relu) MXSS_F(false, true); else MXSS_F(false, false); }
+    });
+#undef MXSS_F
+#undef MXSS
+    CN_LAUNCH_CHECK("cn_mx_scale_shift_act");
     return CN_OK;
 }

@@ -4,6 +4,7 @@ for serving, and the backward passes that read 8-bit activation checkpoints.
     q  = mx.quantize(x, "e4m3" | "e2m1");  y = mx.dequantize(q)
     w4 = mx.pack_weight(weight);           y = mx.linear(x, w4, bias, residual, relu=True)                   # no-grad (serving)
     ck = mx.checkpoint(x, sign_of=y);      dw, db = mx.linear_wgrad(dy, ck, bias=True)
+    y, ck = mx.scale_shift_act(x, scale, shift, residual, relu=True)                                          # y and x's checkpoint at once
                                            dx, dgamma, dbeta, dres = mx.batch_norm_act_bwd(dy, ck, gamma, mean, invstd)
 
 Tensors are [..., channels] in torch.bfloat16 or torch.float32 (NHWC activations of the other operators, or rows of a linear layer);
@@ -145,6 +146,22 @@ def checkpoint(x, sign_of=None):
     """x [..., C] -> e4m3 MXTensor for the backward pass: 8.25 bits a value instead of 16 or 32.  sign_of: the tensor (x's shape and
     dtype) whose positive entries a ReLU let through; one bit of each is kept with the codes."""
     return _quantize(x, "e4m3", sign_of, "mx.checkpoint")
+
+
+def scale_shift_act(x, scale, shift, residual=None, relu=False):
+    """-> (y, ck): y = act(x * scale + shift + residual) per channel (scale, shift fp32 [C]) and ck = checkpoint(x, sign_of=y if relu), in one
+    pass over x: a normalisation's forward apply that keeps what its backward (`batch_norm_act_bwd`) needs."""
+    x, dt = _tensor(x, "mx.scale_shift_act")
+    dev, one = x.device, (x.shape[-1],)
+    scale = _like(scale, dev, one, torch.float32, "mx.scale_shift_act: scale")
+    shift = _like(shift, dev, one, torch.float32, "mx.scale_shift_act: shift")
+    if residual is not None:
+        residual = _like(residual, dev, x.shape, x.dtype, "mx.scale_shift_act: residual")
+    y, q = torch.empty_like(x), MXTensor(x.shape, x.dtype, "e4m3", dev, bool(relu))
+    codes, scales, signs = q._pointers()
+    launch("cn_mx_scale_shift_act", x.get_device(), x.data_ptr(), _ptr(residual), scale.data_ptr(), shift.data_ptr(), y.data_ptr(), codes,
+           scales, signs, q.rows, x.shape[-1], 1 if relu else 0, dt)
+    return y, q
 
 
 def _quantize(x, fmt, sign_of, what):

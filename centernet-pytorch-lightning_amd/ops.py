@@ -1005,29 +1005,6 @@ class StemConvFn(Function):
 
 
 # ------------------------------------------------------------------------------------------------ batch norm
-def _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part):
-    """-> (y, stats [4][C] = mean, invstd, scale, shift) of a training-mode BatchNorm2d + residual + ReLU; part: see BatchNormActFn"""
-    C = x.shape[-1]
-    npix = x.numel() // C
-    y = torch.empty_like(x)
-    stats = torch.empty((4, C), dtype=torch.float32, device=x.device)     # mean, invstd, scale, shift
-    mean, invstd, ss = stats[0], stats[1], stats[2:]
-    ws, n = _bn_ws(npix, C, x.device)
-    if part is not None and BnStats.fused:
-        clear = BnStats.retire(part)          # one launch: the apply kernel reduces the sink, and zeroes the one consumed before it
-        call("cn_bn_train_fwd_sink", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-             part, part.shape[0], clear, clear.numel() if clear is not None else 0, npix, C, BN_MOMENTUM, BN_EPS, int(relu),
-             dtype_code(x.dtype))
-    elif part is not None:
-        call("cn_bn_train_fwd_stats", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-             part, part.shape[0], npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
-        BnStats.release(part)                 # handed back all-zero
-    else:
-        call("cn_bn_train_fwd", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
-             npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
-    return y, stats
-
-
 class BatchNormActFn(Function):
     """Training-mode BatchNorm2d + optional residual add + optional ReLU (one fused apply pass)."""
 
@@ -1035,7 +1012,24 @@ class BatchNormActFn(Function):
     def forward(ctx, x, gamma, beta, running_mean, running_var, residual, relu, part=None):
         """part: the statistics sink the kernel that produced x filled in its epilogue (BnStats) — x is then read once, by the
         apply pass, instead of twice"""
-        y, stats = _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part)
+        C = x.shape[-1]
+        npix = x.numel() // C
+        y = torch.empty_like(x)
+        stats = torch.empty((4, C), dtype=torch.float32, device=x.device)     # mean, invstd, scale, shift
+        mean, invstd, ss = stats[0], stats[1], stats[2:]
+        ws, n = _bn_ws(npix, C, x.device)
+        if part is not None and BnStats.fused:
+            clear = BnStats.retire(part)          # one launch: the apply kernel reduces the sink, and zeroes the one consumed before it
+            call("cn_bn_train_fwd_sink", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+                 part, part.shape[0], clear, clear.numel() if clear is not None else 0, npix, C, BN_MOMENTUM, BN_EPS, int(relu),
+                 dtype_code(x.dtype))
+        elif part is not None:
+            call("cn_bn_train_fwd_stats", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+                 part, part.shape[0], npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
+            BnStats.release(part)                 # handed back all-zero
+        else:
+            call("cn_bn_train_fwd", x, residual, y, gamma.detach(), beta.detach(), running_mean, running_var, mean, invstd, ss,
+                 npix, C, BN_MOMENTUM, BN_EPS, int(relu), dtype_code(x.dtype), ws, n)
         # ReLU backward mask: without a residual input it is recomputed from x and the saved affine (y is not re-read)
         need_y = relu and residual is not None
         ctx.save_for_backward(x, y if need_y else None, gamma, stats)
@@ -1095,13 +1089,23 @@ class BatchNormActFn(Function):
 
 class BatchNormCkptFn(Function):
     """BatchNormActFn with an 8-bit backward: what is kept of the input is its e4m3 checkpoint (and, behind a ReLU, one sign bit of each
-    output), 8.25 - 9.25 bits a value instead of 16 / 32 — and the output need not be kept for the mask either.  The forward result is
-    BatchNormActFn's, bit for bit."""
+    output), 8.25 - 9.25 bits a value instead of 16 / 32 — and the output need not be kept for the mask either.  The checkpoint is written
+    by the pass that applies the statistics; the forward arithmetic is BatchNormActFn's."""
 
     @staticmethod
     def forward(ctx, x, gamma, beta, running_mean, running_var, residual, relu, part=None):
-        y, stats = _bn_train_fwd(x, gamma, beta, running_mean, running_var, residual, relu, part)
-        ck = mx.checkpoint(x, sign_of=y if relu else None)
+        C = x.shape[-1]
+        npix = x.numel() // C
+        stats = torch.empty((4, C), dtype=torch.float32, device=x.device)     # mean, invstd, scale, shift
+        if part is not None:
+            call("cn_bn_finalize_sink", part, part.shape[0], gamma.detach(), beta.detach(), running_mean, running_var, stats[0], stats[1],
+                 stats[2:], npix, C, BN_MOMENTUM, BN_EPS)
+            BnStats.release(part)                 # handed back all-zero
+        else:
+            ws, n = _bn_ws(npix, C, x.device)
+            call("cn_bn_train_stats", x, gamma.detach(), beta.detach(), running_mean, running_var, stats[0], stats[1], stats[2:], npix, C,
+                 BN_MOMENTUM, BN_EPS, dtype_code(x.dtype), ws, n)
+        y, ck = mx.scale_shift_act(x, stats[2], stats[3], residual, relu)
         ctx.save_for_backward(ck.buffer, gamma, stats)
         ctx.ck_meta = ck.meta
         ctx.beta_ref = beta

@@ -237,6 +237,10 @@ int cn_bn_train_fwd(const void* x, const void* residual, void* y, const float* g
                     float* running_mean, float* running_var, float* save_mean, float* save_invstd,
                     float* save_scale_shift, int64_t npix, int C, float momentum, float eps, int relu, int dtype,
                     void* ws, size_t ws_bytes, void* stream);
+/* the statistics half of cn_bn_train_fwd alone (mean / invstd / running stats / scale | shift), no apply pass */
+int cn_bn_train_stats(const void* x, const float* gamma, const float* beta, float* running_mean, float* running_var, float* save_mean,
+                      float* save_invstd, float* save_scale_shift, int64_t npix, int C, float momentum, float eps, int dtype, void* ws,
+                      size_t ws_bytes, void* stream);
 /* y = act(x*scale[c] + shift[c] [+ residual])  (eval-mode BN when it cannot be folded into a conv) */
 int cn_scale_shift_act(const void* x, const void* residual, void* y, const float* scale, const float* shift,
                        int64_t npix, int C, int relu, int dtype, void* stream);
@@ -560,6 +564,10 @@ int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const
 size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype);
 int cn_mx_linear_wgrad(const void* dy, const void* codes, const void* scales, float* dw, float* db, int accumulate, int64_t rows,
                        int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream);
+/* y = act(x * scale[c] + shift[c] [+ residual]) (cn_scale_shift_act's arithmetic, any C) and x's e4m3 checkpoint in the same pass; signs (null
+ * without relu): bits of the stored y > 0.  y may not be x or residual. */
+int cn_mx_scale_shift_act(const void* x, const void* residual, const float* scale, const float* shift, void* y, void* codes, void* scales,
+                          void* signs, int64_t rows, int C, int relu, int dtype, void* stream);
 /* backward of y = [relu](gamma * (x - mean) * invstd + beta [+ residual]) with batch statistics, from an e4m3 checkpoint of x; signs:
  * the ReLU's sign bits (null: no ReLU).  dres (may be null): gradient of the residual input, plus racc (may be null). */
 size_t cn_mx_bn_bwd_bytes(int64_t rows, int C, int dtype);

@@ -188,6 +188,50 @@ def test_checkpoint_signs(dt, rows, C):
     assert ck.nbytes() == rows * (-(-C // 32)) * (32 + 1 + 4)
 
 
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("relu,residual", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("rows,C", [(1, 1), (3, 8), (65, 80), (9, 77), (300, 64), (2000, 264), (5003, 12), (2, 3000), (40000, 32)])
+def test_scale_shift_act(dt, relu, residual, rows, C):
+    """y within its roundings (a product and a sum at once, a sum, the result's), and the checkpoint mx.checkpoint would have made of x and y"""
+    x, res = rnd((rows, C), 1, dt), rnd((rows, C), 2, dt) if residual else None
+    scale, shift = rnd((C,), 3, F32), rnd((C,), 4, F32)
+    y, ck = mx().scale_shift_act(x, scale, shift, res, relu)
+    terms = [f64(x) * f64(scale), np.broadcast_to(f64(shift), x.shape), f64(res) if residual else np.zeros(x.shape)]
+    want = terms[0] + terms[1] + terms[2]
+    want = np.maximum(want, 0) if relu else want
+    within(y, want, half_step(dt) * np.abs(want) + 3 * U * sum(np.abs(t) for t in terms), "y")
+    again = mx().checkpoint(x, sign_of=y if relu else None)
+    assert ck.meta == again.meta and torch.equal(ck.buffer, again.buffer)
+    x[0, 0], x[-1, -1] = float("nan"), float("inf")                        # what is no number stays in its block
+    y2, ck = mx().scale_shift_act(x, scale, shift, res, relu)
+    again = mx().checkpoint(x, sign_of=y2 if relu else None)
+    assert torch.equal(ck.buffer, again.buffer)
+    same = torch.ones(rows, C, dtype=torch.bool, device=DEV)
+    same[0, 0] = same[-1, -1] = False
+    assert torch.equal(y2[same], y[same])
+    if C % 8 == 0:                                                         # the layers' own kernel
+        from centernet_amd import ops
+        assert np.array_equal(f64(ops.scale_shift_act(x, scale, shift, res, relu)), f64(y2), equal_nan=True)
+
+
+def test_scale_shift_act_tiny_values_and_refusals():
+    x = torch.full((4, 64), 2.0 ** -130, device=DEV)
+    y, ck = mx().scale_shift_act(x, torch.full((64,), 2.0 ** -18, device=DEV), torch.zeros(64, device=DEV), None, True)
+    assert torch.equal(ck.buffer, mx().checkpoint(x, sign_of=y).buffer)   # subnormal outputs, kept or flushed, agree with their signs
+    xb = torch.full((4, 64), 2.0 ** -126, device=DEV, dtype=BF)
+    y, ck = mx().scale_shift_act(xb, torch.full((64,), 2.0 ** -20, device=DEV), torch.zeros(64, device=DEV), None, True)
+    assert torch.equal(ck.buffer, mx().checkpoint(xb, sign_of=y).buffer)   # 2^-146 is nothing in 16 bits: not positive
+    y, ck = mx().scale_shift_act(x[:0], x[0], x[0])
+    assert y.shape == (0, 64) and ck.nbytes() == 0
+    v = torch.ones(64, device=DEV)
+    for bad in (lambda: mx().scale_shift_act(x, v[:32], v), lambda: mx().scale_shift_act(x, v, v.bfloat16()), lambda: mx().scale_shift_act(x, v, v.cpu()),
+                lambda: mx().scale_shift_act(x, v, v, x[:2]), lambda: mx().scale_shift_act(x, v, v, x.bfloat16())):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="not on the GPU"):
+        mx().scale_shift_act(x.cpu(), v, v)
+
+
 # ------------------------------------------------------------------------------------------------ product
 LINEAR = [(1, 1, 1), (1, 32, 32), (1, 2048, 512), (2, 64, 80), (31, 16, 64), (33, 77, 5), (64, 100, 200), (65, 513, 130), (129, 208, 65),
           (200, 1100, 300), (130, 4096, 260), (67, 4500, 70), (300, 2100, 100), (5, 9000, 40), (128, 512, 1024), (1000, 64, 64), (257, 256, 2048), (20000, 72, 4), (40, 2056, 3), (50001, 200, 264), (49153, 33, 130)]
@@ -370,7 +414,8 @@ def _pass(x, w4, bias, dy, gamma, mean, invstd):
     m = mx()
     y = m.linear(x, w4, bias, relu=True)
     ck = m.checkpoint(x, sign_of=x)
-    return (y, m.dequantize(m.quantize(y, "e4m3")), *m.linear_wgrad(dy, ck, bias=True), *m.batch_norm_act_bwd(x, ck, gamma, mean, invstd, residual=True))
+    a, cka = m.scale_shift_act(y, bias, bias, y, relu=True)
+    return (y, a, m.dequantize(cka), m.dequantize(m.quantize(y, "e4m3")), *m.linear_wgrad(dy, ck, bias=True), *m.batch_norm_act_bwd(x, ck, gamma, mean, invstd, residual=True))
 
 
 def _inputs(seed, rows=3000, K=96, N=72):

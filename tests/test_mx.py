@@ -53,6 +53,16 @@ ODD = ctypes.c_void_p(4100)
     ("cn_mx_linear_wgrad", (P, P, P, None, None, 0, 8, 32, 32, 1, P, 1 << 30, None)),
     ("cn_mx_linear_wgrad", (P, ODD, P, P, None, 0, 8, 32, 32, 1, P, 1 << 30, None)),
     ("cn_mx_bn_bwd", (P, P, P, None, P, P, P, P, None, None, P, P, 0, 0, 32, 1, P, 1 << 30, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, None, -1, 32, 0, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, None, 4, 65537, 0, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, None, 4, 32, 1, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, P, 4, 32, 0, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, ODD, P, None, 4, 32, 0, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, None, P, P, P, None, 4, 32, 0, 1, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, None, 4, 32, 0, 5, None)),
+    ("cn_bn_train_stats", (P, P, P, None, None, P, P, P, 0, 32, 0.1, 1e-5, 1, P, 1 << 30, None)),
+    ("cn_bn_train_stats", (P, P, P, None, None, P, P, P, 64, 20, 0.1, 1e-5, 1, P, 1 << 30, None)),
+    ("cn_bn_train_stats", (P, P, P, None, None, P, P, None, 64, 32, 0.1, 1e-5, 1, P, 1 << 30, None)),
     ("cn_mx_bn_bwd", (P, P, P, None, P, P, P, P, None, P, P, P, 0, 8, 32, 1, P, 1 << 30, None)),
     ("cn_mx_bn_bwd", (P, P, P, None, None, P, P, P, None, None, P, P, 0, 8, 32, 1, P, 1 << 30, None)),
 ])
