@@ -159,12 +159,10 @@ class BatchNorm2d(nn.BatchNorm2d):
         if self.training:
             self._pending += 1
             ops.WeightsEpoch.bump()              # running_mean / running_var are about to change through raw pointers
-            if self.ckpt8 and torch.is_grad_enabled():
-                return ops.batch_norm_act(x, self, residual, relu, ckpt=True)
             if (defer and BN_DEFER and residual is None and x.dtype == torch.bfloat16 and x.shape[-1] == 16
                     and getattr(x, "_bn_part", None) is not None and getattr(x, "_cn_pre", None) is None):
-                return ops.batch_norm_defer(x, self, relu)
-            return ops.batch_norm_act(x, self, residual, relu)
+                return ops.batch_norm_defer(x, self, relu)         # (keeps x once for this layer and its consumer: less than two checkpoints)
+            return ops.batch_norm_act(x, self, residual, relu, ckpt=self.ckpt8 and torch.is_grad_enabled())
         s, b = self.folded()
         return ops.scale_shift_act(x, s, b, residual, relu)
 
@@ -227,7 +225,7 @@ class StemConv(nn.Module):
 
 def stem_bn_act(stem, bn, img, dtype, relu=True, defer=False):
     """stem conv -> BN -> ReLU; one fused kernel in eval / no-grad mode.  defer: see BatchNorm2d.forward."""
-    if (defer and BN_DEFER and STEM_BN_FUSED and bn.training and not bn.ckpt8 and dtype == torch.bfloat16 and stem.weight.shape[0] == 16
+    if (defer and BN_DEFER and STEM_BN_FUSED and bn.training and dtype == torch.bfloat16 and stem.weight.shape[0] == 16
             and stem.weight.shape[2] == 7 and stem.padding == 3 and stem.weight.shape[1] <= 3 and ops.BnStats.enabled):
         # the BN behind the stem lives entirely in the neighbouring kernels (ops.StemBnDeferFn)
         bn._pending += 1
@@ -316,7 +314,8 @@ class MaxPool2d(nn.Module):
 def use_checkpoints(module, on=True):
     """Training with 8-bit activation checkpoints: every Conv2d and BatchNorm2d under `module` keeps its input in e4m3 (one scale per 32
     channels) and a ReLU's mask in bits, instead of the bf16 / fp32 tensors.  The forward pass is unchanged; gradients are those of
-    the layers at the rounded inputs.  (The task heads, DCN and transposed convolutions keep what they kept.)  -> layers switched"""
+    the layers at the rounded inputs.  (The task heads, DCN and transposed convolutions keep what they kept, and so do the bf16 layers
+    whose batch norm is applied by their consumer: they keep one tensor between the two.)  -> layers switched"""
     n = 0
     for m in module.modules():
         if isinstance(m, (Conv2d, BatchNorm2d)):

@@ -229,6 +229,26 @@ def test_model_with_checkpoints(arch):
     assert kept[True] < 0.8 * kept[False]
 
 
+def test_which_layers_keep_checkpoints():
+    """bf16 layers whose batch norm is applied by their consumer keep one tensor between the two, all others checkpoints"""
+    x, tgt = _batch()
+    names = {}
+    for ck in (False, True):
+        total, _ = (model := _detector("dla_34", ck, BF)).loss(model(x), tgt)
+        seen, todo, names[ck] = set(), [total.grad_fn], []
+        while todo:
+            node = todo.pop()
+            if node is not None and node not in seen:
+                seen.add(node)
+                names[ck].append(type(node).__name__)
+                todo += [n for n, _ in node.next_functions]
+    count = lambda ck, what: names[ck].count(what + "Backward")     # noqa: E731
+    for kind in ("BnDeferFn", "StemBnDeferFn"):
+        assert count(True, kind) == count(False, kind) > 0
+    assert count(True, "BatchNormCkptFn") == count(False, "BatchNormActFn") > 30 and count(True, "BatchNormActFn") == 0
+    assert count(True, "Conv2dCkptFn") > 20
+
+
 @pytest.mark.parametrize("arch", ["dla_34", "res_101"])
 def test_training_steps_with_checkpoints(arch):
     """captured bf16 training steps: replays stay finite and the weights that move are the plain model's (a model may own unused ones)"""
