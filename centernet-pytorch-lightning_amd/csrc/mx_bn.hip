@@ -7,7 +7,7 @@
 // x8 is what the e4m3 codes stand for.  The sums need every row before the first dx, so dy and the codes are read twice: 2 x 3.16
 // bytes per bf16 element in, 2 (4 with a residual input) out.  A thread owns eight channels and walks rows, so the sums and the
 // coefficients stay in registers; partial sums are joined in a fixed order (results do not depend on the schedule).
-// Bound by memory: 262144 x 256 bf16, with ReLU, sums 37 us (211 MB, 5.7 TB/s), finish 5, dx 74 (345 MB, 4.7 TB/s: reads and writes mixed);
+// Bound by memory: 262144 x 256 bf16, with ReLU, sums 39 us (211 MB, 5.4 TB/s), finish 5, dx 74 (345 MB, 4.7 TB/s: reads and writes mixed);
 // 512 x 512 7.1 us in one launch.
 #include "mx_common.h"
 
@@ -314,7 +314,8 @@ __device__ static inline float mx_stored(float v, const float*) { return v; }
 __device__ static inline float mx_stored(float v, const bf16_t*) { return bf2f(f2bf(v)); }
 
 // Forward: y = act(x scale + shift (+ residual)) and x's checkpoint in one pass (separately the checkpoint reads x and y again).  A thread
-// owns eight channels, filler included, and walks rows with its coefficients in registers; a quad of lanes is one block of 32.
+// owns eight channels, filler included, and walks rows with its coefficients in registers; a quad of lanes is one block of 32.  Bound by
+// memory: 262144 x 256 bf16 with ReLU 75 us (345 MB, 4.6 TB/s), apply and checkpoint apart 103; 65536 x 64 8.3 | 12.0.
 template <typename T, bool RES, bool RELU, bool FULL>
 __global__ __launch_bounds__(256) void mx_scale_shift_act_kernel(const MxBnGeom g, const T* __restrict__ x, const T* __restrict__ res,
                                                                  const float* __restrict__ scale, const float* __restrict__ shift,
@@ -476,7 +477,7 @@ extern "C" int cn_mx_scale_shift_act(const void* x, const void* residual, const 
     MxBnGeom g{nullptr, nullptr, nullptr, nullptr, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 2, 0};
     while (g.lg < 5 && (1 << g.lg) < g.cpr) ++g.lg;
     const int tiles = cdiv(g.cpr, 1 << g.lg), nrl = 256 >> g.lg;
-    int deep = 8;                                                 // (rows a thread: as in the backward pass)
+    int deep = 8;                                                 // rows a thread, by the backward pass's rule
     while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
     g.per = (int64_t)deep * nrl;
     CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_scale_shift_act: too many rows");
