@@ -162,7 +162,9 @@ class BatchNorm2d(nn.BatchNorm2d):
             if (defer and BN_DEFER and residual is None and x.dtype == torch.bfloat16 and x.shape[-1] == 16
                     and getattr(x, "_bn_part", None) is not None and getattr(x, "_cn_pre", None) is None):
                 return ops.batch_norm_defer(x, self, relu)         # (keeps x once for this layer and its consumer: less than two checkpoints)
-            return ops.batch_norm_act(x, self, residual, relu, ckpt=self.ckpt8 and torch.is_grad_enabled())
+            if self.ckpt8 and torch.is_grad_enabled():
+                return ops.batch_norm_act(x, self, residual, relu, ckpt=True)
+            return ops.batch_norm_act(x, self, residual, relu)
         s, b = self.folded()
         return ops.scale_shift_act(x, s, b, residual, relu)
 
