@@ -6,7 +6,7 @@
 // keeps them there while it walks all its columns, so x is read from memory once whatever N is; the weights stream from L2 in
 // fragment order (1 KB contiguous per 32 columns x 64 channels).  K beyond what LDS holds is taken in chunks.
 // Bound by memory: 65536x256x1024 with its residual 57 us (302 MB, 5.3 TB/s, the rate of a copy), 65536x1024x256 41 us (168 MB, 4.1 TB/s:
-// reading x alone takes 28, quantising, products and stores overlap with it in part), 1x2048x512 4.4 us (latency of one row's K).
+// reading x alone takes 28, quantising, products and stores overlap with it in part), 1x2048x512 4.2 us (latency of one row's K).
 #include "mx_common.h"
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
@@ -80,12 +80,13 @@ struct MxLinGeom {
 // two steps of NJ weight tiles
 template <int NJ> struct MxLinB { u32x4_t f[2][NJ]; };
 
-// 32 x 32 NJ outputs per wave; WM x WN waves over rows and columns, WK over the channels (few rows: the launch would be short of waves
+// 32 x 32 NJ outputs per wave; WM x WN waves over rows and columns, or WK over the channels (few rows: the launch would be short of waves
 // otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows.  RT > 1 (K <= 256): a wave takes
 // RT row tiles one after the other with the weights of its columns in registers (read from L2 half as often: 65536x256x1024 69 -> 63 us).
 template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN, bool resident>
-__global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
-    static_assert(WM * WN * WK == 4 && (WK == 1 || WK == 4) && (RT == 1 || (WK == 1 && resident)), "four waves");
+__global__ __launch_bounds__(64 * WM * WN * WK, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
+    static_assert((WK == 1 ? WM * WN == 4 : WM * WN == 1) && (RT == 1 || (WK == 1 && resident)), "rows and columns, or channels");
+    constexpr int NT = 64 * WM * WN * WK;
     constexpr int BM = 32 * RT * WM, EPN = 32 * NJ, EPP = EPN + 4;         // EPP: floats per staged output row (rows on different banks)
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = WK > 1 ? 0 : wave / WN, wn = WK > 1 ? 0 : wave % WN, wk = WK > 1 ? wave : 0;
@@ -94,9 +95,9 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
     const T* __restrict__ X = reinterpret_cast<const T*>(g.x) + m0 * g.K;
 
     // Quantise channels 64 s0 .. 64 s1 of the workgroup's rows into LDS (rows behind the last stay as they are: what they give is not
-    // stored).  A thread's chunks are 256 apart; row and channel are carried along (multiplications cost four times an addition).
+    // stored).  A thread's chunks are NT apart; row and channel are carried along (multiplications cost four times an addition).
     auto stage = [&](int s0, int s1) {
-        const int d = (s1 - s0) * 8, dq = 256 / d, dr = 256 - dq * d;          // 8-channel chunks per row (uniform)
+        const int d = (s1 - s0) * 8, dq = NT / d, dr = NT - dq * d;          // 8-channel chunks per row (uniform)
         const uint32_t step = (uint32_t)(dq * g.K + dr * 8), wrap = (uint32_t)(g.K - d * 8);
         constexpr int U = sizeof(T) == 2 && WK == 1 ? 8 : 4;                   // loads in flight per thread; WK > 1: and as many again
         struct At { int row, pc; uint32_t ofs; };
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 #pragma unroll
                     for (int e = 0; e < 16; ++e) ep[(wk * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * EPP + j * 32 + (lane & 31)] = acc[j][e];
                 __syncthreads();
-                for (int r = tid / LPR; r < rows; r += 256 / LPR) {
+                for (int r = tid / LPR; r < rows; r += NT / LPR) {
                     if (g.res) rv[0].template load<FULLN>(reinterpret_cast<const T*>(g.res), (m0 + r) * g.N + nc, left, true, g.N);
                     float v[8];
 #pragma unroll
@@ -335,7 +336,8 @@ __global__ __launch_bounds__(256, resident && sizeof(T) == 2 ? 4 : 2) void mx_li
 template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN>
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
     constexpr int BM = 32 * RT * WM, EPP = 32 * NJ + 4;
-    const int ep = (WK > 1 ? 4 * 32 : 4 * 16) * EPP * 4;
+    constexpr int NT = 64 * WM * WN * WK;
+    const int ep = (WK > 1 ? WK * 32 : 4 * 16) * EPP * 4;
     // LDS holds all channels of the rows where they fit, else a chunk at a time
     int chunk = g.S;
     auto bytes = [&](int c) {
@@ -369,20 +371,26 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
         if (dev < 64) attr[dev] = true;
     }
     const dim3 grid((unsigned)mt, (unsigned)split);
-    if (RT > 1 || chunk >= g.S) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, 256, smem, st>>>(g);
-    else if constexpr (RT == 1) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, 256, smem, st>>>(g);
+    if (RT > 1 || chunk >= g.S) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, NT, smem, st>>>(g);
+    else if constexpr (RT == 1) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, NT, smem, st>>>(g);
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
 }
 // Which waves do what, us (bf16, M x K x N):
 //   K split over the waves, 32 x 32 a workgroup | columns over the waves, 32 x 256: 64x1440x64 8.8 | 10.3, 512x2048x512 10.9 | 13.0,
-//     2048x64x256 5.1 | 5.5, 20000x1440x8 15.4 | 17.5; the other way 512x512x2048 9.3 | 6.6, 8192x512x64 6.9 | 6.4, 8192x1024x256 15.2 | 10.0
+//     2048x64x256 5.1 | 5.5, 20000x1440x8 15.4 | 17.5, and there over four | eight waves (one workgroup a compute unit at most and more than
+//     16384 values for it to quantise): 41x1872x82 10.7 | 9.1, 256x4096x256 18.4 | 14.4, 1x2048x512 5.0 | 5.0, 8x2048x512 5.8 | 5.6, 32x256x64 4.9 | 5.2, 296x752x1106 8.5 |
+//     9.1 (sixteen: 9.1, 13.7, 5.4, 6.0, 11.8); the other way 512x512x2048 9.3 | 6.6, 8192x512x64 6.9 | 6.4, 8192x1024x256 15.2 | 10.0
 //   rows over the waves, 128 x 64 | 64 x 128 | 32 x 256: 65536x64x64 7.4 | 8.7 | 11.4, 65536x256x128 16.4 | 13.3 | 14.7, 65536x512x64
 //     17.5 | 17.4 | 16.4, 65536x1024x256 111 | 53 | 44
 //   32 x 256 | two row tiles, 64 x 256: 65536x256x1024 with its residual 69 | 63, 262144x64x256 52 | 41, 32768x256x512 14.4 | 15.7
 template <typename T, bool FULLK, bool FULLN>
 static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
-    if (g.N <= 32 || (g.M + 31) / 32 * cdiv(g.N, 32) <= 512) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
+    const int64_t wgs = (g.M + 31) / 32 * cdiv(g.N, 32);
+    if (g.N <= 32 || wgs <= 512) {
+        if (wgs <= 256 && (g.M < 32 ? g.M : 32) * g.K > 16384) return mxl_launch<T, 1, 1, 1, 1, 8, FULLK, FULLN>(g, st);
+        return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
+    }
     if (g.N <= 64 && g.K <= 256) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
     if (g.N <= 128 && g.K <= 256) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
     if (g.K <= 256 && g.M >= 49152) return mxl_launch<T, 2, 2, 1, 4, 1, FULLK, FULLN>(g, st);
