@@ -21,6 +21,40 @@ STEM_BN_FUSED = not (os.environ.get("CN_DISABLE_STEM_BN_FUSED") or os.environ.ge
 BN_DEFER = not (os.environ.get("CN_DISABLE_BN_DEFER") or os.environ.get("CN_DISABLE_CONV_C16R") or os.environ.get("CN_DISABLE_WGRAD_C16"))
 
 
+class Derived:
+    """What a layer makes of its parameters for the no-grad path, kept until they change: an entry answers for the tensors it was made from
+    (it holds them, so no other takes their place) at their versions, in its `ops.WeightsEpoch`.
+
+    The replays of a graph read what its capture was given, so that stays for the layer's life (a capture at other weights keeps one more).
+    What a capture itself makes exists only once the graph has run: it lies in the graph's memory and is not kept here."""
+    __slots__ = ("entry", "captured")
+
+    def __init__(self):
+        self.entry = None            # (key, value, made)
+        self.captured = []           # entries that a captured graph reads
+
+    @classmethod
+    def of(cls, layer, name):
+        d = layer.__dict__.get(name)
+        if d is None:
+            d = layer.__dict__[name] = cls()
+        return d
+
+    def get(self, key, made, make):
+        """make() for `key` and the tensors `made` (or None among them), or what it gave the last time"""
+        key = (key, ops.WeightsEpoch.value, *(None if t is None else t._version for t in made))
+        e = self.entry
+        hit = e is not None and e[0] == key and all(a is b for a, b in zip(e[2], made))
+        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+            if not hit:
+                return make()
+            if all(c is not e for c in self.captured):
+                self.captured.append(e)
+        elif not hit:
+            e = self.entry = (key, make(), made)
+        return e[1]
+
+
 class Conv2d(nn.Module):
     ckpt8 = False           # `use_checkpoints`: keep the input in 8 bits for the backward pass
     mx4 = False             # `use_mxfp4`: the no-grad forward as a 4-bit product (1x1, stride 1)
@@ -94,12 +128,8 @@ class Conv2d(nn.Module):
         return ops._igemm(x, c["wp"], c["b"], residual, Co, KH, KW, self.stride, self.padding, False, relu, OH, OW, out_dtype)
 
     def _mx_weight(self, x, scale, shift):
-        """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels; kept while
-        the tensors they were made from are these, unchanged (versions; the entry holds the tensors, so no other takes their place)"""
-        made = (self.weight, self.bias, scale, shift)
-        key = (x.shape[-1], x.device, ops.WeightsEpoch.value, *(None if t is None else t._version for t in made))
-        hit = self.__dict__.get("_mx_cache")
-        if hit is None or hit[0] != key or any(a is not b for a, b in zip(hit[3], made)):
+        """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels"""
+        def make():
             Co, Ci = self.weight.shape[:2]
             with torch.no_grad():
                 w = torch.zeros(ops.rup(Co, 16), x.shape[-1], dtype=torch.float32, device=x.device)
@@ -109,10 +139,9 @@ class Conv2d(nn.Module):
                     b[:Co] = self.bias if scale is None else self.bias * scale
                 if shift is not None:
                     b[:Co] += shift
-            hit = (key, mx.pack_weight(w), b, made)
-            if not torch.cuda.is_current_stream_capturing():       # (what a capture packs exists only once the graph has run)
-                self._mx_cache = hit
-        return hit[1], hit[2]
+            return mx.pack_weight(w), b
+
+        return Derived.of(self, "_mx_cache").get((x.shape[-1], x.device), (self.weight, self.bias, scale, shift), make)
 
     def infer_nchw(self, x):
         """No-grad 1x1 conv + bias straight into the public fp32 NCHW layout (a head's last layer); packed weights cached as in `infer`."""

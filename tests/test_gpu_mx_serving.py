@@ -1,0 +1,40 @@
+"""What the layers keep for the no-grad path, under captured graphs and streams on the GPU."""
+import pytest
+import torch
+
+from tests.test_gpu_mx import BF, DEV, F32, rnd
+from tests.test_gpu_mx_layers import hnn, img, ops
+
+pytestmark = pytest.mark.gpu
+
+
+def _refill(n=64):
+    """take what the allocator has free and fill it with something else"""
+    return [torch.full((1 << 14,), 0x7f, dtype=torch.uint8, device=DEV) for _ in range(n)]
+
+
+def test_replays_read_the_weights_they_were_captured_with():
+    """warm-up, capture, then new weights and an eager call, which makes the layer pack again: the graph's own weights stay"""
+    n = hnn()
+    conv, bn = n.Conv2d(64, 64, 1).to(DEV), n.BatchNorm2d(64).to(DEV).eval()
+    x = img((2, 8, 8, 64), 1, BF)
+    n.use_mxfp4(conv)
+    with torch.no_grad():
+        want = n.conv_bn_act(conv, bn, x)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = n.conv_bn_act(conv, bn, x)
+        for rep in range(3):
+            if rep == 1:
+                conv.weight.copy_(rnd((64, 64, 1, 1), 5, F32))
+            else:
+                ops().WeightsEpoch.bump()
+            eager = n.conv_bn_act(conv, bn, x)
+            assert torch.equal(eager, want) == (rep < 1)
+            junk = _refill()
+            y.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want), rep
+            del junk
