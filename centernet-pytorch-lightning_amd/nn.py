@@ -23,14 +23,15 @@ BN_DEFER = not (os.environ.get("CN_DISABLE_BN_DEFER") or os.environ.get("CN_DISA
 
 class Derived:
     """What a layer makes of its parameters for the no-grad path, kept until they change: an entry answers for the tensors it was made from
-    (it holds them, so no other takes their place) at their versions, in its `ops.WeightsEpoch`.
+    (it holds them and their memory, so no other takes their place) at their versions and addresses (`.data` assigned anew keeps the
+    version), in its `ops.WeightsEpoch`.
 
     The replays of a graph read what its capture was given, so that stays for the layer's life (a capture at other weights keeps one more).
     What a capture itself makes exists only once the graph has run: it lies in the graph's memory and is not kept here."""
     __slots__ = ("entry", "captured")
 
     def __init__(self):
-        self.entry = None            # (key, value, made)
+        self.entry = None            # (key, value, made, aliases of these that hold their memory)
         self.captured = []           # entries that a captured graph reads
 
     @classmethod
@@ -42,7 +43,7 @@ class Derived:
 
     def get(self, key, made, make):
         """make() for `key` and the tensors `made` (or None among them), or what it gave the last time"""
-        key = (key, ops.WeightsEpoch.value, *(None if t is None else t._version for t in made))
+        key = (key, ops.WeightsEpoch.value, *(None if t is None else (t._version, t.data_ptr()) for t in made))
         e = self.entry
         hit = e is not None and e[0] == key and all(a is b for a, b in zip(e[2], made))
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
@@ -51,7 +52,7 @@ class Derived:
             if all(c is not e for c in self.captured):
                 self.captured.append(e)
         elif not hit:
-            e = self.entry = (key, make(), made)
+            e = self.entry = (key, make(), made, [None if t is None else t.detach() for t in made])
         return e[1]
 
 

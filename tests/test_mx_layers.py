@@ -3,6 +3,7 @@ import gc
 import os
 import weakref
 
+import numpy as np
 import pytest
 import torch
 
@@ -63,3 +64,26 @@ def test_what_a_capture_packs_is_not_kept(packing):
     first = conv._mx_weight(x, None, None)[0]
     packing["capturing"] = False
     assert conv._mx_weight(x, None, None)[0] is not first
+
+
+def test_new_data_in_the_same_parameter_is_packed_anew(packing):
+    """`p.data = t` (what `module.to` does) changes neither the parameter nor its version"""
+    conv, x = hnn().Conv2d(32, 16, 1, bias=True), torch.zeros(1, 1, 1, 32)
+    w, b = conv._mx_weight(x, None, None)
+    assert conv._mx_weight(x, None, None)[0] is w
+    conv.weight.data = conv.weight.data + 1
+    w2, b2 = conv._mx_weight(x, None, None)
+    assert not torch.equal(w2.packed, w.packed)
+    conv.bias.data = conv.bias.data + 1
+    assert torch.equal(conv._mx_weight(x, None, None)[1], b2 + 1)
+    data = np.zeros((16, 32, 1, 1), np.float32)
+    first = weakref.ref(data)
+    conv.weight.data = torch.from_numpy(data)
+    del data
+    conv._mx_weight(x, None, None)
+    conv.weight.data = torch.ones(16, 32, 1, 1)
+    gc.collect()
+    assert first() is not None                                     # or the next data could lie where the first did
+    conv._mx_weight(x, None, None)
+    gc.collect()
+    assert first() is None
