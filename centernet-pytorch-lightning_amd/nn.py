@@ -21,17 +21,46 @@ STEM_BN_FUSED = not (os.environ.get("CN_DISABLE_STEM_BN_FUSED") or os.environ.ge
 BN_DEFER = not (os.environ.get("CN_DISABLE_BN_DEFER") or os.environ.get("CN_DISABLE_CONV_C16R") or os.environ.get("CN_DISABLE_WGRAD_C16"))
 
 
+class _Entry:
+    """one value of a `Derived` and what makes it safe to hand out"""
+    __slots__ = ("key", "value", "made", "memory", "tensors", "device", "stream", "done")
+
+    def __init__(self, key, value, made):
+        self.key, self.value, self.made = key, value, made
+        self.memory = [None if t is None else t.detach() for t in made]        # (the memory of `made`: no other tensor gets their addresses)
+        self.tensors = [getattr(t, "packed", t) for t in value if t is not None]
+        self.device, self.stream, self.done = made[0].get_device(), None, None
+        if self.device >= 0:
+            self.stream = torch._C._cuda_getCurrentRawStream(self.device)
+            self.done = torch.cuda.current_stream(self.device).record_event()
+
+    def follow(self):
+        """The current stream may be another than the one that makes the value: wait for that, and let the memory not be used again before
+        this stream's work is done."""
+        if self.device < 0 or torch._C._cuda_getCurrentRawStream(self.device) == self.stream:
+            return
+        here = torch.cuda.current_stream(self.device)
+        if self.done is not None:
+            if self.done.query():
+                self.done = None
+            else:
+                here.wait_event(self.done)
+        for t in self.tensors:
+            t.record_stream(here)
+
+
 class Derived:
     """What a layer makes of its parameters for the no-grad path, kept until they change: an entry answers for the tensors it was made from
     (it holds them and their memory, so no other takes their place) at their versions and addresses (`.data` assigned anew keeps the
-    version), in its `ops.WeightsEpoch`.
+    version), in its `ops.WeightsEpoch`, on any stream.
 
     The replays of a graph read what its capture was given, so that stays for the layer's life (a capture at other weights keeps one more).
-    What a capture itself makes exists only once the graph has run: it lies in the graph's memory and is not kept here."""
+    What a capture itself makes exists only once the graph has run: it lies in the graph's memory and is not kept here.  (A capture does not
+    wait for the stream that made an entry: `torch.cuda.graph` has synchronised before it begins.)"""
     __slots__ = ("entry", "captured")
 
     def __init__(self):
-        self.entry = None            # (key, value, made, aliases of these that hold their memory)
+        self.entry = None
         self.captured = []           # entries that a captured graph reads
 
     @classmethod
@@ -42,18 +71,21 @@ class Derived:
         return d
 
     def get(self, key, made, make):
-        """make() for `key` and the tensors `made` (or None among them), or what it gave the last time"""
+        """make() (a tuple of tensors, packed weights or None) for `key` and the tensors `made` (the first is one, others may be None), or what
+        it gave the last time"""
         key = (key, ops.WeightsEpoch.value, *(None if t is None else (t._version, t.data_ptr()) for t in made))
         e = self.entry
-        hit = e is not None and e[0] == key and all(a is b for a, b in zip(e[2], made))
+        hit = e is not None and e.key == key and all(a is b for a, b in zip(e.made, made))
         if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
             if not hit:
                 return make()
             if all(c is not e for c in self.captured):
                 self.captured.append(e)
-        elif not hit:
-            e = self.entry = (key, make(), made, [None if t is None else t.detach() for t in made])
-        return e[1]
+        elif hit:
+            e.follow()
+        else:
+            e = self.entry = _Entry(key, make(), made)
+        return e.value
 
 
 class Conv2d(nn.Module):

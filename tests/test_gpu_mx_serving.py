@@ -38,3 +38,40 @@ def test_replays_read_the_weights_they_were_captured_with():
             torch.cuda.synchronize()
             assert torch.equal(y, want), rep
             del junk
+
+
+def _delay():
+    """some milliseconds of the current stream"""
+    torch.cuda._sleep(20_000_000)
+
+
+def test_weights_packed_on_one_stream_are_used_on_another():
+    """the layer packs on a stream that is far behind; another stream's call waits for that, and its own work may outlive the entry"""
+    n = hnn()
+    conv = n.Conv2d(256, 256, 1, bias=True).to(DEV)
+    n.use_mxfp4(conv)
+    x = img((1, 16, 16, 256), 1, BF)
+    ws = [rnd((256, 256, 1, 1), 5 + i, F32) for i in range(3)]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        wants = []
+        for w in ws:
+            conv.weight.copy_(w)
+            wants.append(conv(x))
+        for i in (0, 1, 2, 1):
+            conv.weight.copy_(ws[i])
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                _delay()
+                first = conv(x)
+            with torch.cuda.stream(b):
+                second = conv(x)
+                _delay()
+                third = conv(x)                                    # queued when the entry goes
+            with torch.cuda.stream(a):
+                ops().WeightsEpoch.bump()
+                conv(x)
+                junk = _refill()
+            torch.cuda.synchronize()
+            del junk
+            assert all(torch.equal(y, wants[i]) for y in (first, second, third)), i
