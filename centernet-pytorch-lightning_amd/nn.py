@@ -63,6 +63,10 @@ class Derived:
         self.entry = None
         self.captured = []           # entries that a captured graph reads
 
+    def __reduce__(self):
+        """a copy of the layer begins anew: its parameters are others, and start at version 0 again"""
+        return Derived, ()
+
     @classmethod
     def of(cls, layer, name):
         d = layer.__dict__.get(name)
@@ -102,7 +106,6 @@ class Conv2d(nn.Module):
             self.bias = nn.Parameter(torch.empty(cout).uniform_(-bound, bound))
         else:
             self.register_parameter("bias", None)
-        self._cache = {}
 
     def __getstate__(self):
         """copies and pickles pack their 4-bit weights again: a copied parameter starts at version 0"""
@@ -138,16 +141,15 @@ class Conv2d(nn.Module):
 
     def infer_key(self, x, scale=None, shift=None):
         """-> the cache entry {wp: packed (folded) weights, b: folded bias} for x's dtype and the current parameter versions"""
-        key = (x.dtype, self.weight._version, None if self.bias is None else self.bias._version, ops.WeightsEpoch.value,
-               None if scale is None else (scale.data_ptr(), scale._version))
-        hit = self._cache.get("k")
-        if hit != key:
+        def make():
             wp = ops.pack_weight(self.weight, 1, x.dtype, scale)
             b = self.bias.detach() if self.bias is not None else None
             if shift is not None:
                 b = shift if b is None else (b * scale + shift)   # tiny [Co] host-side fold (once per weight version)
-            self._cache = {"k": key, "wp": wp, "b": b}
-        return self._cache
+            return wp, b
+
+        wp, b = Derived.of(self, "_packed").get(x.dtype, (self.weight, self.bias, scale, shift), make)
+        return {"wp": wp, "b": b}
 
     def infer(self, x, scale, shift, residual, relu, out_dtype=None):
         """No-grad path: y = act(conv(x)*scale + shift + residual); packed (folded) weights are cached."""
@@ -184,8 +186,8 @@ class Conv2d(nn.Module):
             out = torch.empty((N, self.weight.shape[0], H, W), dtype=torch.float32, device=x.device)
             ops.call("cn_nhwc_to_nchw", y, out, N, self.weight.shape[0], H, W, ld, ops.dtype_code(y.dtype))
             return out
-        self.infer_key(x)
-        return ops.conv1x1_to_nchw(x, self._cache["wp"], self._cache["b"], self.weight.shape[0])
+        c = self.infer_key(x)
+        return ops.conv1x1_to_nchw(x, c["wp"], c["b"], self.weight.shape[0])
 
 
 class BatchNorm2d(nn.BatchNorm2d):
@@ -195,7 +197,6 @@ class BatchNorm2d(nn.BatchNorm2d):
     def __init__(self, c):
         super().__init__(c, momentum=ops.BN_MOMENTUM)
         self._pending = 0
-        self._fold = None
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         if self._pending:
@@ -206,14 +207,13 @@ class BatchNorm2d(nn.BatchNorm2d):
     def folded(self):
         """(scale, shift) fp32 of the eval-mode affine; cached per buffer/parameter version and per `ops.WeightsEpoch` (the
         optimizer and the training-mode kernel update parameters / running statistics behind `_version`'s back)."""
-        key = (self.weight._version, self.bias._version, self.running_mean._version, self.running_var._version,
-               ops.WeightsEpoch.value)
-        if self._fold is None or self._fold[0] != key:
+        def make():
             with torch.no_grad():
                 scale = self.weight * torch.rsqrt(self.running_var + self.eps)   # [C] vectors, once per weight version
                 shift = self.bias - self.running_mean * scale
-            self._fold = (key, scale.contiguous(), shift.contiguous())
-        return self._fold[1], self._fold[2]
+            return scale.contiguous(), shift.contiguous()
+
+        return Derived.of(self, "_folded").get(self.eps, (self.weight, self.bias, self.running_mean, self.running_var), make)
 
     def forward(self, x, residual=None, relu=True, defer=False):
         """defer: the caller guarantees that the ONLY consumer of the result is a 3x3 Conv2d with 16 input channels (DLA base_layer ->
@@ -252,11 +252,8 @@ def cat_conv_bn_act(conv, bn, xs, residual=None, relu=True):
     s, b = bn.folded()                              # eval: BN folded into the packed weights, one launch
     if conv.mx4:
         return conv.infer(ops.concat(list(xs)), s, b, residual, relu)
-    key = ("cat", xs[0].dtype, conv.weight._version, ops.WeightsEpoch.value, s.data_ptr(), s._version)
-    if conv._cache.get("k") != key:
-        conv._cache = {"k": key, "wp": ops.pack_weight(conv.weight, 1, xs[0].dtype, s), "b": b}
-    return ops.conv1x1_cat_raw([t.contiguous() for t in xs], conv._cache["wp"], conv._cache["b"], residual,
-                               conv.weight.shape[0], relu)
+    c = conv.infer_key(xs[0], s, b)
+    return ops.conv1x1_cat_raw([t.contiguous() for t in xs], c["wp"], c["b"], residual, conv.weight.shape[0], relu)
 
 
 def conv_bn_act(conv, bn, x, residual=None, relu=True, defer=False):
@@ -344,24 +341,22 @@ class DCN(nn.Module):
         nn.init.zeros_(self.conv_offset_mask.weight)
         nn.init.zeros_(self.conv_offset_mask.bias)
 
-        self._cache = {}
-
     def forward(self, x, bn_stats=False):
         y = ops.DCNv2Fn.apply(x, self.weight, self.bias, self.conv_offset_mask.weight, self.conv_offset_mask.bias, bn_stats)
         return ops.BnStats.pop(y) if bn_stats else y
 
     def infer(self, x, scale, shift, relu):
         """No-grad path with the following BN folded in: offset conv -> sampling -> ONE 1x1 GEMM (+shift, ReLU)."""
-        key = (x.dtype, self.weight._version, self.bias._version, ops.WeightsEpoch.value, scale.data_ptr(), scale._version)
-        if self._cache.get("k") != key:
-            wp = ops.pack_weight(self.weight, 1, x.dtype, scale)
-            self._cache = {"k": key, "wp": wp, "b": (self.bias.detach() * scale + shift).contiguous()}
+        def make():
+            return ops.pack_weight(self.weight, 1, x.dtype, scale), (self.bias.detach() * scale + shift).contiguous()
+
+        wp, b = Derived.of(self, "_packed").get(x.dtype, (self.weight, self.bias, scale, shift), make)
         N, H, W, Ci = x.shape
         om = self.conv_offset_mask.infer(x, None, None, None, False, out_dtype=torch.float32)
         Co = self.weight.shape[0]
         cp = ops.rup(Co, 16)
         y = torch.empty((N, H, W, cp), dtype=x.dtype, device=x.device) if cp == Co else ops.zeros((N, H, W, cp), x.dtype, x.device)
-        ops.call("cn_dcn_fwd", x, om, self._cache["wp"], self._cache["b"], y, N, H, W, Ci, Ci, Co, cp, om.shape[-1], int(relu),
+        ops.call("cn_dcn_fwd", x, om, wp, b, y, N, H, W, Ci, Ci, Co, cp, om.shape[-1], int(relu),
                  ops.dtype_code(x.dtype))
         return y
 

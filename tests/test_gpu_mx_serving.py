@@ -75,3 +75,77 @@ def test_weights_packed_on_one_stream_are_used_on_another():
             torch.cuda.synchronize()
             del junk
             assert all(torch.equal(y, wants[i]) for y in (first, second, third)), i
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_replays_of_the_plain_path_read_the_weights_they_were_captured_with(dt):
+    """convolution + batch norm, a root over several sources and a deformable convolution, in bf16 / fp32"""
+    n = hnn()
+    torch.manual_seed(0)
+    conv, root, bn, dcn = n.Conv2d(64, 64, 3, 1, 1).to(DEV), n.Conv2d(128, 64, 1).to(DEV), n.BatchNorm2d(64).to(DEV).eval(), n.DCN(64, 64).to(DEV)
+    x = img((2, 16, 16, 64), 1, dt)
+    one, zero = torch.ones(64, device=DEV), torch.zeros(64, device=DEV)
+
+    def forward():
+        y = n.conv_bn_act(conv, bn, x)
+        return n.cat_conv_bn_act(root, bn, [x, y]), bn(y), dcn.infer(x, one, zero, True)
+
+    with torch.no_grad():
+        wants = forward()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ys = forward()
+        for rep in range(3):
+            if rep == 1:
+                for m in (conv, root, dcn):
+                    m.weight.mul_(2)
+                bn.running_mean.add_(1)
+            else:
+                ops().WeightsEpoch.bump()
+            eager = forward()
+            assert all(torch.equal(a, b) == (rep < 1) for a, b in zip(eager, wants))
+            junk = _refill()
+            for y in ys:
+                y.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(ys, wants)), rep
+            del junk
+
+
+def test_the_plain_path_captured_before_any_eager_call():
+    n = hnn()
+    conv, bn = n.Conv2d(64, 64, 3, 1, 1).to(DEV), n.BatchNorm2d(64).to(DEV).eval()
+    x = img((2, 8, 8, 64), 1, BF)
+    with torch.no_grad():
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = n.conv_bn_act(conv, bn, x)
+        eager = n.conv_bn_act(conv, bn, x)
+        for _ in range(3):
+            y.fill_(float("nan"))
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+            assert torch.equal(n.conv_bn_act(conv, bn, x), eager)
+
+
+def test_the_plain_path_on_two_streams():
+    n = hnn()
+    conv, bn = n.Conv2d(64, 64, 3, 1, 1).to(DEV), n.BatchNorm2d(64).to(DEV).eval()
+    x = img((1, 16, 16, 64), 1, BF)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.no_grad():
+        for i in range(3):
+            conv.weight.mul_(1.5)
+            bn.running_mean.add_(0.25)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(a):
+                _delay()
+                first = n.conv_bn_act(conv, bn, x)
+            with torch.cuda.stream(b):
+                second = n.conv_bn_act(conv, bn, x)
+            torch.cuda.synchronize()
+            assert torch.equal(first, second) and torch.equal(first, n.conv_bn_act(conv, bn, x))

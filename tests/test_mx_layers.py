@@ -87,3 +87,87 @@ def test_new_data_in_the_same_parameter_is_packed_anew(packing):
     conv._mx_weight(x, None, None)
     gc.collect()
     assert first() is None
+
+
+# ------------------------------------------------------------------------------------------------ the bf16 / fp32 path
+def _fill(bn, seed):
+    g = torch.Generator().manual_seed(seed)
+    return {k: v if k == "num_batches_tracked" else torch.rand(v.shape, generator=g) + 0.5 for k, v in bn.state_dict().items()}
+
+
+def _folded(sd):
+    scale = sd["weight"] / torch.sqrt(sd["running_var"] + 1e-5)
+    return scale, sd["bias"] - sd["running_mean"] * scale
+
+
+def test_a_copy_folds_its_own_batch_norm():
+    """copied parameters start at version 0; loading a state dict brings them to the version at which the first was folded"""
+    import copy
+    import pickle
+    bn = hnn().BatchNorm2d(8)
+    bn.load_state_dict(_fill(bn, 1), assign=True)
+    with torch.no_grad():
+        for t in (bn.weight, bn.bias, bn.running_mean, bn.running_var):
+            t.mul_(1)                                              # version 1
+    bn.folded()
+    for other in (copy.deepcopy(bn), pickle.loads(pickle.dumps(bn))):
+        sd = _fill(bn, 2)
+        other.load_state_dict(sd)
+        for got, want in zip(other.folded(), _folded(sd)):
+            assert torch.allclose(got, want, rtol=1e-5)
+    for seed in (3, 4):                                            # another parameter in the old one's place, and other data in the same
+        sd = _fill(bn, seed)
+        bn.load_state_dict(sd, assign=True)
+        for got, want in zip(bn.folded(), _folded(sd)):
+            assert torch.allclose(got, want, rtol=1e-5)
+    sd = {k: v.clone() for k, v in bn.state_dict().items()}
+    bn.running_mean.data = bn.running_mean.data + 1
+    sd["running_mean"] += 1
+    for got, want in zip(bn.folded(), _folded(sd)):
+        assert torch.allclose(got, want, rtol=1e-5)
+
+
+def _packs(monkeypatch):
+    from centernet_amd import ops
+    monkeypatch.setattr(ops, "pack_weight", lambda w, mode, dtype, scale=None: w.detach().clone() if scale is None else w.detach() * scale.view(-1, 1, 1, 1))
+
+
+def test_a_copy_packs_its_own_weights(monkeypatch):
+    import copy
+    _packs(monkeypatch)
+    conv, x = hnn().Conv2d(4, 6, 3), torch.zeros(1)
+    with torch.no_grad():
+        conv.load_state_dict({"weight": torch.randn(6, 4, 3, 3)}, assign=True)
+        conv.weight.mul_(1)
+    assert torch.equal(conv.infer_key(x)["wp"], conv.weight) and conv.infer_key(x)["wp"] is conv.infer_key(x)["wp"]
+    other, new = copy.deepcopy(conv), torch.randn(6, 4, 3, 3)
+    other.load_state_dict({"weight": new})
+    assert other.weight._version == conv.weight._version and torch.equal(other.infer_key(x)["wp"], new)
+    for _ in range(2):
+        new = torch.randn(6, 4, 3, 3)
+        conv.load_state_dict({"weight": new}, assign=True)
+        assert torch.equal(conv.infer_key(x)["wp"], new)
+    conv.weight.data = new + 1
+    assert torch.equal(conv.infer_key(x)["wp"], new + 1)
+
+
+def test_graphs_keep_packed_and_folded_weights_too(packing, monkeypatch):
+    _packs(monkeypatch)
+    conv, bn, x = hnn().Conv2d(4, 6, 3), hnn().BatchNorm2d(6), torch.zeros(1)
+    packing["capturing"] = True
+    made = bn.folded()                                             # without a warm-up: in the graph's memory, not for eager calls
+    packing["capturing"] = False
+    s, b = bn.folded()
+    assert s is not made[0]
+    wp = conv.infer_key(x, s, b)["wp"]
+    packing["capturing"] = True
+    assert bn.folded()[0] is s and conv.infer_key(x, s, b)["wp"] is wp
+    packing["capturing"] = False
+    kept = [weakref.ref(t) for t in (s, b, wp)]
+    del s, b, wp, made
+    with torch.no_grad():
+        conv.weight.add_(1)
+        bn.weight.add_(1)
+    conv.infer_key(x, *bn.folded())
+    gc.collect()
+    assert all(r() is not None for r in kept)
