@@ -470,8 +470,8 @@ extern "C" int cn_mx_scale_shift_act(const void* x, const void* residual, const 
                                      void* scales, void* signs, int64_t rows, int C, int relu, int dtype, void* stream) {
     CN_CHECK_ARG(rows >= 0 && C >= 1 && C <= MX_MAX_C && rows <= ((int64_t)1 << 40) / C, "cn_mx_scale_shift_act: rows %lld, channels %d", (long long)rows, C);
     CN_CHECK_ARG(dtype == CN_F32 || dtype == CN_BF16, "cn_mx_scale_shift_act: bad dtype %d", dtype);
+    if (rows == 0) return CN_OK;                                  // (an empty buffer's pointers are null)
     CN_CHECK_ARG((signs != nullptr) == (relu != 0), "cn_mx_scale_shift_act: signs come with relu");
-    if (rows == 0) return CN_OK;
     CN_CHECK_ARG(x && scale && shift && y && codes && scales, "cn_mx_scale_shift_act: null pointer");
     CN_CHECK_ARG(((uintptr_t)codes & 15) == 0, "cn_mx_scale_shift_act: codes must be 16-byte aligned");
     MxBnGeom g{nullptr, nullptr, nullptr, nullptr, rows, C, cdiv(C, MX_BLOCK) * 4, cdiv(C, MX_BLOCK), 0, 2, 0};

@@ -149,3 +149,13 @@ def test_the_plain_path_on_two_streams():
                 second = n.conv_bn_act(conv, bn, x)
             torch.cuda.synchronize()
             assert torch.equal(first, second) and torch.equal(first, n.conv_bn_act(conv, bn, x))
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+def test_scale_shift_act_of_no_rows(dt):
+    from centernet_amd import mx
+    v = torch.ones(48, device=DEV)
+    for relu in (False, True):
+        x = torch.empty(2, 0, 48, dtype=dt, device=DEV)
+        y, ck = mx.scale_shift_act(x, v, v, x, relu)
+        assert y.shape == (2, 0, 48) and ck.has_signs == relu and ck.nbytes() == 0

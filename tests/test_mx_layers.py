@@ -171,3 +171,10 @@ def test_graphs_keep_packed_and_folded_weights_too(packing, monkeypatch):
     conv.infer_key(x, *bn.folded())
     gc.collect()
     assert all(r() is not None for r in kept)
+
+
+# ------------------------------------------------------------------------------------------------ entry points
+def test_scale_shift_act_of_no_rows(lib):
+    """an empty checkpoint's buffers are null, those of its sign bits too"""
+    for relu in (0, 1):
+        assert lib.cn_mx_scale_shift_act(None, None, None, None, None, None, None, None, 0, 32, relu, 1, None) == 0
