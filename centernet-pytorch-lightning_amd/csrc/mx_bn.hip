@@ -443,6 +443,12 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
     const int tiles = cdiv(cdiv(C, 8), 1 << g.lg);
     const int nrl = 256 >> g.lg;
     CN_CHECK_ARG(tiles <= 65535, "cn_mx_bn_bwd: too many channels");
+    // apply pass: eight rows a thread (its coefficients are loaded once), fewer where that would leave less than two workgroups a compute unit (us, this
+    // rule | always two rows | always eight: 4515x28 11.7 | 12.0 | 14.7, 8192x256 13.2 | 13.2 | 14.1, 262144x256 110 | 113 | 110)
+    int deep = 8;
+    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
+    g.per = (int64_t)deep * nrl;
+    CN_CHECK_ARG(mx_grid_fits((rows + g.per - 1) / g.per, 256), "cn_mx_bn_bwd: too many rows for one launch");
     MXBN_GO(mx_bn_sums_kernel, , dim3(groups, tiles), g, mean, part);
     CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     const MxBnTail t{coef, part, gamma, invstd, dgamma, dbeta, 1.f / (float)rows, groups, accumulate};
@@ -451,12 +457,6 @@ extern "C" int cn_mx_bn_bwd(const void* dy, const void* codes, const void* scale
         mx_bn_finish_kernel<<<cdiv(C, 4), 256, 0, st>>>(part, groups, C, ld, t.inv_rows, gamma, invstd, coef, dgamma, dbeta, accumulate);
         CN_LAUNCH_CHECK("cn_mx_bn_bwd");
     }
-    // eight rows a thread (its coefficients are loaded once), fewer where that would leave less than two workgroups a compute unit (us, this
-    // rule | always two rows | always eight: 4515x28 11.7 | 12.0 | 14.7, 8192x256 13.2 | 13.2 | 14.1, 262144x256 110 | 113 | 110)
-    int deep = 8;
-    while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
-    g.per = (int64_t)deep * nrl;
-    CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_bn_bwd: too many rows");
     const int ng = cdiv(rows, g.per);
     if (joined) MXBN_GO(mx_bn_apply_kernel, MXBN_COMMA true, dim3(ng, tiles), g, mean, t, (T*)dx, (T*)dres, (const T*)racc);
     else MXBN_GO(mx_bn_apply_kernel, MXBN_COMMA false, dim3(ng, tiles), g, mean, t, (T*)dx, (T*)dres, (const T*)racc);
@@ -480,7 +480,7 @@ extern "C" int cn_mx_scale_shift_act(const void* x, const void* residual, const 
     int deep = 8;                                                 // rows a thread, by the backward pass's rule
     while (deep > 1 && (rows + deep * nrl - 1) / (deep * nrl) * tiles < 512) deep /= 2;
     g.per = (int64_t)deep * nrl;
-    CN_CHECK_ARG((rows + g.per - 1) / g.per < ((int64_t)1 << 31), "cn_mx_scale_shift_act: too many rows");
+    CN_CHECK_ARG(mx_grid_fits((rows + g.per - 1) / g.per, 256), "cn_mx_scale_shift_act: too many rows for one launch");
     const dim3 grid(cdiv(rows, g.per), tiles);
     hipStream_t st = (hipStream_t)stream;
 #define MXSS(RES, RELU, FULL)                                                                                                          \

@@ -234,6 +234,9 @@ __device__ static inline void mx_values_e2m1(uint32_t c, float s, float (&v)[8])
     p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);         v[6] = p.x * s; v[7] = p.y * s;
 }
 
+// a launch has less than 2^32 threads along x (the runtime's limit); what would need more is refused before anything runs
+static inline bool mx_grid_fits(int64_t workgroups, int threads) { return workgroups < ((int64_t)1 << 32) / threads; }
+
 // n / d for n * d < 2^32 by one high multiplication (m = ceil(2^32 / d); d = 1 has m = 0)
 struct MxDiv { uint32_t d, m; };
 static inline MxDiv mx_div(uint32_t d) { return MxDiv{d, d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d)}; }

@@ -352,7 +352,7 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     const int smem = g.ep_ofs + ep;
     g.t32 = cdiv(g.N, 32);
     const int64_t mt = (g.M + BM - 1) / BM;
-    if (mt >= ((int64_t)1 << 31)) { cn_set_error("cn_mx_linear_fwd: too many rows"); return CN_EINVAL; }
+    CN_CHECK_ARG(mx_grid_fits(mt, NT), "cn_mx_linear_fwd: too many rows for one launch");
     const int passes = cdiv(g.t32, NJ * WN);
     // one workgroup walks all columns of its rows unless that leaves less than four workgroups a compute unit.  us, never split | this rule |
     // one pass a workgroup: 512x512x2048 16.8 | 6.5 | 6.8, 4096x512x2048 19.3 | 13.1 | 13.1, 16384x256x1024 14.8 | 14.9 | 17.1,

@@ -97,7 +97,7 @@ extern "C" int cn_mx_quantize(const void* x, void* codes, void* scales, const vo
     // 5.0, 65536x256 11.3 | 10.5, 262144x256 39.5 | 38.1
     const bool many = chunks >= (int64_t)256 * 4 * 1024, full = C % 8 == 0;
     const int64_t grid = (chunks + 256 * (many ? 4 : 1) - 1) / (256 * (many ? 4 : 1));
-    CN_CHECK_ARG(grid < ((int64_t)1 << 31), "cn_mx_quantize: tensor too large");
+    CN_CHECK_ARG(mx_grid_fits(grid, 256), "cn_mx_quantize: too many rows for one launch");
 #define MX_Q(FMT, SIGNS, U, FULL)                                                                                                      \
     mx_quantize_kernel<T, FMT, SIGNS, U, FULL><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>((const T*)x, (const T*)sign_src,       \
         (uint8_t*)codes, (uint8_t*)scales, (uint8_t*)signs, chunks, C, mx_div(cpr))
@@ -122,7 +122,7 @@ extern "C" int cn_mx_dequantize(const void* codes, const void* scales, void* out
     const int64_t chunks = rows * cpr;
     const int per = chunks >= (int64_t)256 * 4 * 1024 ? 4 : 1;      // us, one | four: 4096x256 4.1 | 4.5, 262144x256 33.6 | 32.0
     const int64_t grid = (chunks + 256 * per - 1) / (256 * per);
-    CN_CHECK_ARG(grid < ((int64_t)1 << 31), "cn_mx_dequantize: tensor too large");
+    CN_CHECK_ARG(mx_grid_fits(grid, 256), "cn_mx_dequantize: too many rows for one launch");
     CN_DISPATCH_DTYPE(dtype, T, {
         if (fmt == CN_MX_E2M1)
             mx_dequantize_kernel<T, CN_MX_E2M1><<<(unsigned)grid, 256, 0, (hipStream_t)stream>>>((const uint8_t*)codes, (const uint8_t*)scales, (T*)out, chunks, C, mx_div(cpr), per);

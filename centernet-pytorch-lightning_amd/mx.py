@@ -8,7 +8,8 @@ for serving, and the backward passes that read 8-bit activation checkpoints.
                                            dx, dgamma, dbeta, dres = mx.batch_norm_act_bwd(dy, ck, gamma, mean, invstd)
 
 Tensors are [..., channels] in torch.bfloat16 or torch.float32 (NHWC activations of the other operators, or rows of a linear layer);
-any channel count from 1 to 65536 and any number of rows, zero included where a result is defined.  Nothing here is recorded by autograd
+any channel count from 1 to 65536 and any number of rows, zero included where a result is defined (what one launch's 2^32 threads do not
+cover is refused: from 2^32 blocks of 32 channels when quantising, from 2^29 rows of a product).  Nothing here is recorded by autograd
 (the layers' autograd functions call these).  Non-contiguous inputs are copied.
 Work is enqueued on the current stream of the tensors' device; nothing synchronises and scratch comes from torch's allocator, so every
 call can be captured into a graph and two captured graphs share no scratch.  Results do not depend on the launch (sums have a fixed

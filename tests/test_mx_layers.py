@@ -178,3 +178,20 @@ def test_scale_shift_act_of_no_rows(lib):
     """an empty checkpoint's buffers are null, those of its sign bits too"""
     for relu in (0, 1):
         assert lib.cn_mx_scale_shift_act(None, None, None, None, None, None, None, None, 0, 32, relu, 1, None) == 0
+
+
+P = 4096                            # never dereferenced: every call below is refused on the host
+
+
+@pytest.mark.parametrize("name,args", [
+    ("cn_mx_quantize", (P, P, P, None, None, 1 << 33, 1, 1, 1, None)),
+    ("cn_mx_dequantize", (P, P, P, 1 << 33, 1, 0, 1, None)),
+    ("cn_mx_linear_fwd", (P, P, None, None, P, 1 << 30, 16, 8, 0, 1, None)),
+    ("cn_mx_linear_fwd", (P, P, None, None, P, 1 << 33, 64, 64, 0, 0, None)),
+    ("cn_mx_bn_bwd", (P, P, P, None, P, P, P, P, None, None, P, P, 0, 1 << 36, 1, 1, P, 1 << 30, None)),
+    ("cn_mx_scale_shift_act", (P, None, P, P, P, P, P, P, 1 << 36, 1, 1, 1, None)),
+])
+def test_more_threads_than_a_launch_has_are_refused(lib, name, args):
+    assert getattr(lib, name)(*args) == -1
+    error = lib.cn_last_error().decode()
+    assert name in error and "one launch" in error
