@@ -135,9 +135,11 @@ class Conv2d(nn.Module):
     def with_skip(self, x, bn_stats=False):
         """-> (conv(x), x) for a residual connection around this conv: the skip path's gradient is added in the epilogue of this
         conv's data-gradient kernel (training; otherwise just the pair)."""
-        if torch.is_grad_enabled() and x.requires_grad and self.stride == 1 and not self.ckpt8:
+        if torch.is_grad_enabled() and x.requires_grad and self.stride == 1:
+            if self.ckpt8:
+                return ops.conv2d_ckpt(x, self.weight, self.bias, self.stride, self.padding, bn_stats, passthrough=True)
             return ops.conv2d(x, self.weight, self.bias, self.stride, self.padding, False, False, False, True, bn_stats=bn_stats)
-        return self.forward(x, bn_stats=bn_stats), x
+        return self.forward(x), x
 
     def infer_key(self, x, scale=None, shift=None):
         """-> the cache entry {wp: packed (folded) weights, b: folded bias} for x's dtype and the current parameter versions"""

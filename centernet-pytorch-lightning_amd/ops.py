@@ -791,7 +791,7 @@ class Conv2dCkptFn(Function):
     gradient reads the codes themselves; any other shape writes the values out again for the time of its own backward."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, stride, pad, bn_stats=False):
+    def forward(ctx, x, weight, bias, stride, pad, bn_stats=False, passthrough=False):
         Co, Ci, KH, KW = weight.shape
         N, H, W, Cx = x.shape
         assert Cx == rup(Ci, 16), f"conv input has {Cx} channels, weight expects {Ci}"
@@ -805,10 +805,15 @@ class Conv2dCkptFn(Function):
         ctx.bias_ref = bias
         ctx.order = SideGrads.next_order()
         ctx.cell = cell_of(x)
+        if passthrough:
+            ctx.set_materialize_grads(False)
+            return y, x.view_as(x)
         return y
 
     @staticmethod
-    def backward(ctx, dy):
+    def backward(ctx, dy, dskip=None):
+        if dy is None:                                 # only the skip path carried a gradient
+            return ctx.cell.give(dskip) if ctx.cell is not None else dskip, None, None, None, None, None, None
         buffer, weight = ctx.saved_tensors
         ck = None if buffer is None else mx.MXTensor.of(buffer, ctx.ck_meta)
         (stride, pad), bias = ctx.cfg, ctx.bias_ref
@@ -823,8 +828,8 @@ class Conv2dCkptFn(Function):
             dw, db = _ckpt_wgrad(dy, ck, weight, bias, ctx.order)
         else:
             x, rest = mx.dequantize(ck), need[:3]
-        out = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, rest)
-        return (out[0], *(out[1:] if rest[1] else (dw, db)), None, None, None)
+        out = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, rest, dskip)
+        return (out[0], *(out[1:] if rest[1] else (dw, db)), None, None, None, None)
 
 
 def _cat_args(xs):
@@ -2009,7 +2014,10 @@ def weighted_sum(terms, weights):
 def conv2d(x, weight, bias=None, stride=1, pad=0, relu=False, mask_dx=False, defer_relu_bwd=False, passthrough=False, bn_stats=False, pre=None):
     """bn_stats: the output feeds a training-mode BatchNorm — ask the kernel for the batch statistics (BnStats);
     pre: x is a raw conv output whose BN (+ ReLU) the kernels apply on load (batch_norm_defer)"""
-    out = Conv2dFn.apply(x, weight, bias, stride, pad, relu, mask_dx, defer_relu_bwd, passthrough, bn_stats, pre)
+    return _conv_out(x, Conv2dFn.apply(x, weight, bias, stride, pad, relu, mask_dx, defer_relu_bwd, passthrough, bn_stats, pre), passthrough, bn_stats)
+
+
+def _conv_out(x, out, passthrough, bn_stats):
     if bn_stats:
         BnStats.pop(out[0] if passthrough else out)
     if passthrough and cell_of(x) is not None:
@@ -2017,10 +2025,9 @@ def conv2d(x, weight, bias=None, stride=1, pad=0, relu=False, mask_dx=False, def
     return out
 
 
-def conv2d_ckpt(x, weight, bias=None, stride=1, pad=0, bn_stats=False):
+def conv2d_ckpt(x, weight, bias=None, stride=1, pad=0, bn_stats=False, passthrough=False):
     """conv2d whose input is kept in e4m3 for its weight gradient (mx.checkpoint)"""
-    y = Conv2dCkptFn.apply(x, weight, bias, stride, pad, bn_stats)
-    return BnStats.pop(y) if bn_stats else y
+    return _conv_out(x, Conv2dCkptFn.apply(x, weight, bias, stride, pad, bn_stats, passthrough), passthrough, bn_stats)
 
 
 def conv_transpose2d(x, weight, stride=2, pad=1):

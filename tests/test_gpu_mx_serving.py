@@ -159,3 +159,28 @@ def test_scale_shift_act_of_no_rows(dt):
         x = torch.empty(2, 0, 48, dtype=dt, device=DEV)
         y, ck = mx.scale_shift_act(x, v, v, x, relu)
         assert y.shape == (2, 0, 48) and ck.has_signs == relu and ck.nbytes() == 0
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("k,p", [(1, 0), (3, 1)])
+@pytest.mark.parametrize("shared", [False, True])
+def test_identity_around_a_checkpointed_convolution(dt, k, p, shared):
+    """the skip path's gradient joins in the data gradient's epilogue (one rounding in all), as without checkpoints"""
+    n = hnn()
+    conv = n.Conv2d(64, 64, k, 1, p).to(DEV)
+    x = img((2, 8, 8, 64), 1, dt)
+    dy, ds = img((2, 8, 8, 64), 2, dt, 1e-2), img((2, 8, 8, 64), 3, dt, 1e-2)
+    out = {}
+    for ck in (False, True):
+        n.use_checkpoints(conv, ck)
+        xi = x.clone().requires_grad_()
+        xs = ops().share(xi * 1) if shared else xi
+        y, skip = conv.with_skip(xs)
+        assert torch.equal(skip, x) and type(y.grad_fn).__name__.startswith("Conv2dCkptFn") == ck
+        torch.autograd.backward([y, skip], [dy, ds], retain_graph=True)
+        both = xi.grad.clone()
+        xi.grad = None
+        torch.autograd.backward([skip], [ds])                      # the convolution's output unused
+        out[ck] = (y.detach(), both, xi.grad)
+    assert all(torch.equal(a, b) for a, b in zip(out[True], out[False]))
+    assert torch.equal(out[True][2], ds)
