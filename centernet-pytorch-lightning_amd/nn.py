@@ -120,7 +120,7 @@ class Conv2d(nn.Module):
     def forward(self, x, relu=False, mask_dx=False, defer_relu_bwd=False, bn_stats=False):
         """bn_stats: the output goes straight into a training-mode BatchNorm2d (ops.BnStats: statistics from the conv epilogue)"""
         pre = getattr(x, "_cn_pre", None)           # x is a raw conv output whose BN (+ ReLU) is applied by this conv's kernels (ops.BnDeferFn)
-        if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad):
+        if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad or (self.bias is not None and self.bias.requires_grad)):
             if self.ckpt8 and pre is None and not (relu or mask_dx or defer_relu_bwd):
                 return ops.conv2d_ckpt(x, self.weight, self.bias, self.stride, self.padding, bn_stats)
             return ops.conv2d(x, self.weight, self.bias, self.stride, self.padding, relu, mask_dx, defer_relu_bwd, bn_stats=bn_stats, pre=pre)

@@ -704,6 +704,9 @@ def _conv2d_bwd(x, weight, bias_ref, dy, stride, pad, has_bias, mask_dx, cell, o
         SideGrads.submit(SideGrads.wide_if_tail(side_work, order), x, dy, claims=(weight, bias_ref))
     elif needs[1]:
         dw, db = _wgrad_param(x, dy, Co, Ci, KH, KW, stride, pad, want_bias=has_bias and needs[2], pre=pre)
+    elif needs[2] and has_bias:                        # a frozen weight under a bias that is not: x is not needed
+        db = zeros((Co,), torch.float32, dy.device)
+        call("cn_colsum", dy, db, dy.numel() // dy.shape[-1], Co, dy.shape[-1], dtype_code(dy.dtype))
     if needs[0]:
         if pre is not None and mask_dx:
             raise RuntimeError("mask_dx on a conv whose input BN is deferred: the masks would be applied twice")
@@ -795,7 +798,7 @@ class Conv2dCkptFn(Function):
         Co, Ci, KH, KW = weight.shape
         N, H, W, Cx = x.shape
         assert Cx == rup(Ci, 16), f"conv input has {Cx} channels, weight expects {Ci}"
-        ck = _input_checkpoint(x) if any(ctx.needs_input_grad[1:3]) else None          # (a frozen layer keeps nothing)
+        ck = _input_checkpoint(x) if ctx.needs_input_grad[1] else None                 # (a frozen weight needs no input)
         y = _igemm(x, pack_weight(weight, 1, x.dtype), bias, None, Co, KH, KW, stride, pad, False, False, conv_out(H, KH, stride, pad),
                    conv_out(W, KW, stride, pad), bn_stats=bn_stats)
         ctx.save_for_backward(None if ck is None else ck.buffer, weight)
@@ -820,16 +823,13 @@ class Conv2dCkptFn(Function):
         Co, Ci, KH, KW = weight.shape
         need = ctx.needs_input_grad
         dy = dy.contiguous()
-        x, dw, db, rest = ctx.like, None, None, (need[0], False, False)
-        if not need[1]:
-            if need[2]:                                # a frozen weight under a bias that is not
-                db = _wgrad_param(mx.dequantize(ck), dy, Co, Ci, KH, KW, stride, pad, want_bias=True)[1]
-        elif (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
-            dw, db = _ckpt_wgrad(dy, ck, weight, bias, ctx.order)
-        else:
-            x, rest = mx.dequantize(ck), need[:3]
-        out = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, rest, dskip)
-        return (out[0], *(out[1:] if rest[1] else (dw, db)), None, None, None, None)
+        x, wgrads, needs = ctx.like, None, need[:3]
+        if need[1] and (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
+            wgrads, needs = _ckpt_wgrad(dy, ck, weight, bias, ctx.order), (need[0], False, False)
+        elif need[1]:
+            x = mx.dequantize(ck)
+        dx, dw, db = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, needs, dskip)
+        return (dx, *(wgrads or (dw, db)), None, None, None, None)
 
 
 def _cat_args(xs):
@@ -1903,7 +1903,7 @@ class HeadFn(Function):
             hg = _igemm(xg, pack_weight(w1.detach().view(Ch, K, 1, 1), 1, dt), b1.detach(), None, Ch, 1, 1, 1, 0, False, True, 1, R)
             call("cn_head_sparse_gather_rows", hg, x, ind, g, w2c, dhc, None, None, N, M, C, H, W, Ch, hg.shape[-1], Ci, Cx, Cq, 2, dtype_code(dt))
         dw1 = db1 = dw2 = db2 = dx = None
-        if need[1] or need[3]:
+        if any(need[1:5]):
             if SideGrads.usable(w1, b1, w2, b2):
                 def side_work():
                     _wgrad_param(hg, gq, C, Ch, 1, 1, 1, 0, into=w2.grad, db_into=b2.grad)

@@ -1,8 +1,9 @@
 """What the layers keep for the no-grad path, under captured graphs and streams on the GPU."""
+import numpy as np
 import pytest
 import torch
 
-from tests.test_gpu_mx import BF, DEV, F32, rnd
+from tests.test_gpu_mx import BF, DEV, F32, U, f64, rnd, within
 from tests.test_gpu_mx_layers import hnn, img, ops
 
 pytestmark = pytest.mark.gpu
@@ -184,3 +185,48 @@ def test_identity_around_a_checkpointed_convolution(dt, k, p, shared):
         out[ck] = (y.detach(), both, xi.grad)
     assert all(torch.equal(a, b) for a, b in zip(out[True], out[False]))
     assert torch.equal(out[True][2], ds)
+
+
+@pytest.mark.parametrize("dt", [BF, F32])
+@pytest.mark.parametrize("ck", [False, True])
+@pytest.mark.parametrize("k,p,Co", [(1, 0, 24), (3, 1, 32), (1, 0, 2)])
+def test_a_bias_trains_above_a_frozen_weight(dt, ck, k, p, Co):
+    """its gradient is dy's column sums and nothing of the input is kept for it.  Tolerance: 2^-24 of the magnitudes for each of at most
+    72 + 16 additions, whatever their order"""
+    conv = hnn().Conv2d(32, Co, k, 1, p, bias=True).to(DEV)
+    hnn().use_checkpoints(conv, ck)
+    conv.weight.requires_grad_(False)
+    x = img((2, 6, 6, 32), 1, dt).requires_grad_()
+    y = conv(x)
+    assert not ck or y.grad_fn.saved_tensors[0] is None
+    dy = img(tuple(y.shape), 2, dt, 1e-2)
+    dy[..., Co:] = 0
+    y.backward(dy)
+    d = f64(dy)[..., :Co].reshape(-1, Co)
+    within(conv.bias.grad, d.sum(0), 88 * U * np.abs(d).sum(0), "db")
+    assert conv.weight.grad is None and x.grad is not None
+    first, conv.bias.grad = conv.bias.grad, None
+    conv(x.detach()).backward(dy)                                  # nothing but the bias wants a gradient
+    within(conv.bias.grad, f64(first), 2 * 88 * U * np.abs(d).sum(0), "db alone")
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_biases_of_a_head_train_above_frozen_weights(rows):
+    """for a loss over the whole map and for one that gathers a few rows"""
+    from centernet_amd import ops as o
+    torch.manual_seed(0)
+    x = img((2, 16, 16, 64), 1, BF)
+    w1, b1, w2, b2 = rnd((64, 64, 3, 3), 2, F32) * 0.05, rnd((64,), 3, F32), rnd((2, 64, 1, 1), 4, F32), rnd((2,), 5, F32)
+    ind = torch.randint(0, 256, (2, 5), generator=torch.Generator().manual_seed(1)).to(DEV)
+    got = {}
+    for frozen in (False, True):
+        ps = [t.clone().requires_grad_(not (frozen and t.dim() == 4)) for t in (w1, b1, w2, b2)]
+        out = o.HeadFn.apply(x.clone().requires_grad_(), *ps)
+        if rows:
+            o.GatherL1Fn.apply(out, torch.ones(2, 5, dtype=torch.uint8, device=DEV), ind, torch.zeros(2, 5, 2, device=DEV)).backward()
+        else:
+            (out * out).sum().backward()
+        got[frozen] = [p.grad for p in ps]
+    assert got[True][0] is None and got[True][2] is None
+    for i in (1, 3):
+        assert got[True][i] is not None and torch.allclose(got[True][i], got[False][i], rtol=1e-4, atol=1e-4 * float(got[False][i].abs().max()))
