@@ -773,9 +773,9 @@ def _shape_only(t):
     return torch.empty((1,) * len(t.shape), dtype=t.dtype, device=t.device).expand(t.shape)
 
 
-def _ckpt_wgrad(dy, ck, weight, bias, order):
+def _ckpt_wgrad(dy, ck, weight, bias):
     """Weight (+ bias) gradient of a 1x1 convolution from its input's checkpoint: -> (dw, db), or (None, None) when they were deposited
-    in `.grad` on the side stream (inside a TrainStep)"""
+    in `.grad` on the side stream (inside a TrainStep).  Its grid is the operator's own there too: `SideGrads.grid` does not hold it."""
     Co = weight.shape[0]
     if dy.shape[-1] != Co:
         dy = dy[..., :Co].contiguous()
@@ -783,7 +783,7 @@ def _ckpt_wgrad(dy, ck, weight, bias, order):
         def side_work():
             mx.linear_wgrad(dy, ck, into=weight.grad, bias=bias is not None, bias_into=None if bias is None else bias.grad)
             GradReady.note(weight, bias)
-        SideGrads.submit(SideGrads.wide_if_tail(side_work, order), dy, ck.buffer, claims=(weight, bias))
+        SideGrads.submit(side_work, dy, ck.buffer, claims=(weight, bias))
         return None, None
     dw, db = mx.linear_wgrad(dy, ck, bias=bias is not None)
     return dw.view(weight.shape), db
@@ -825,7 +825,7 @@ class Conv2dCkptFn(Function):
         dy = dy.contiguous()
         x, wgrads, needs = ctx.like, None, need[:3]
         if need[1] and (KH, KW, stride, pad) == (1, 1, 1, 0) and ck.shape[-1] == Ci:
-            wgrads, needs = _ckpt_wgrad(dy, ck, weight, bias, ctx.order), (need[0], False, False)
+            wgrads, needs = _ckpt_wgrad(dy, ck, weight, bias), (need[0], False, False)
         elif need[1]:
             x = mx.dequantize(ck)
         dx, dw, db = _conv2d_bwd(x, weight, bias, dy, stride, pad, bias is not None, False, ctx.cell, ctx.order, needs, dskip)
