@@ -10,7 +10,8 @@ for serving, and the backward passes that read 8-bit activation checkpoints.
 Tensors are [..., channels] in torch.bfloat16 or torch.float32 (NHWC activations of the other operators, or rows of a linear layer);
 any channel count from 1 to 65536 and any number of rows, zero included where a result is defined (what one launch's 2^32 threads do not
 cover is refused: from 2^32 blocks of 32 channels when quantising, from 2^29 rows of a product).  Nothing here is recorded by autograd
-(the layers' autograd functions call these).  Non-contiguous inputs are copied.
+(the layers' autograd functions call these): `quantize`, `scale_shift_act` and `linear` refuse inputs that want a gradient while autograd
+records, a checkpoint and the results of the backward passes are constants to it.  Non-contiguous inputs are copied.
 Work is enqueued on the current stream of the tensors' device; nothing synchronises and scratch comes from torch's allocator, so every
 call can be captured into a graph and two captured graphs share no scratch.  Results do not depend on the launch (sums have a fixed
 order).  Layers use these operators through `nn.use_checkpoints` (training) and `nn.use_mxfp4` (no-grad forward).
@@ -119,6 +120,12 @@ def _tensor(t, what):
     return (t if t.is_contiguous() else t.contiguous()), code
 
 
+def _unrecorded(what, *tensors):
+    """an error where autograd would record the call and a tensor wants a gradient: the result would be a constant, without a word"""
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or on detached tensors")
+
+
 def _like(t, device, shape, dtype, what):
     """t contiguous if it is a tensor of that device, shape and type, else an error"""
     if not isinstance(t, torch.Tensor):
@@ -140,18 +147,20 @@ def _fmt(fmt):
 
 def quantize(x, fmt="e4m3"):
     """x [..., C] -> MXTensor.  One pass: x is read once, codes and scales are written."""
+    _unrecorded("mx.quantize", x)
     return _quantize(x, fmt, None, "mx.quantize")
 
 
 def checkpoint(x, sign_of=None):
     """x [..., C] -> e4m3 MXTensor for the backward pass: 8.25 bits a value instead of 16 or 32.  sign_of: the tensor (x's shape and
-    dtype) whose positive entries a ReLU let through; one bit of each is kept with the codes."""
+    dtype) whose positive entries a ReLU let through; one bit of each is kept with the codes.  A copy: no gradient comes back through it."""
     return _quantize(x, "e4m3", sign_of, "mx.checkpoint")
 
 
 def scale_shift_act(x, scale, shift, residual=None, relu=False):
     """-> (y, ck): y = act(x * scale + shift + residual) per channel (scale, shift fp32 [C]) and ck = checkpoint(x, sign_of=y if relu), in one
     pass over x: a normalisation's forward apply that keeps what its backward (`batch_norm_act_bwd`) needs."""
+    _unrecorded("mx.scale_shift_act", x, scale, shift, residual)
     x, dt = _tensor(x, "mx.scale_shift_act")
     dev, one = x.device, (x.shape[-1],)
     scale = _like(scale, dev, one, torch.float32, "mx.scale_shift_act: scale")
@@ -177,7 +186,7 @@ def _quantize(x, fmt, sign_of, what):
 
 
 def dequantize(q, dtype=None):
-    """MXTensor -> the values it stands for, in `dtype` (default: the type it was made from)"""
+    """MXTensor -> the values it stands for, in `dtype` (default: the type it was made from); to autograd a constant"""
     if not isinstance(q, MXTensor):
         raise TypeError(f"mx.dequantize: expected an MXTensor, got {type(q).__name__}")
     dtype = dtype or q.dtype
@@ -213,8 +222,7 @@ def linear(x, weight, bias=None, residual=None, relu=False):
     x's type.  Serving only: an input that wants a gradient is refused (train in bf16, pack the result)."""
     if not isinstance(weight, MXWeight):
         raise TypeError("mx.linear: weight must come from mx.pack_weight")
-    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(bias, "requires_grad", False) or getattr(residual, "requires_grad", False)):
-        raise RuntimeError("mx.linear has no backward pass: call it under torch.no_grad()")
+    _unrecorded("mx.linear", x, bias, residual)
     x, dt = _tensor(x, "mx.linear")
     N, K, dev = weight.out_features, weight.in_features, x.device
     if x.shape[-1] != K:

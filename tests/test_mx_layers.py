@@ -195,3 +195,20 @@ def test_more_threads_than_a_launch_has_are_refused(lib, name, args):
     assert getattr(lib, name)(*args) == -1
     error = lib.cn_last_error().decode()
     assert name in error and "one launch" in error
+
+
+def test_inputs_that_want_a_gradient_are_refused():
+    """where autograd records, a result that is a constant to it would cut the gradient without a word"""
+    from centernet_amd import mx
+    x, v = torch.zeros(4, 32), torch.zeros(32)
+    xg, vg = torch.zeros(4, 32, requires_grad=True), torch.zeros(32, requires_grad=True)
+    calls = [lambda: mx.quantize(xg), lambda: mx.quantize(xg * 2, "e2m1"), lambda: mx.scale_shift_act(xg, v, v), lambda: mx.scale_shift_act(x, vg, v),
+             lambda: mx.scale_shift_act(x, v, vg), lambda: mx.scale_shift_act(x, v, v, xg, True)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="not on the GPU|expected"):       # (taken: the next check speaks)
+            call()
+    for call in (lambda: mx.quantize(xg.detach()), lambda: mx.checkpoint(xg), lambda: mx.checkpoint(x, sign_of=xg)):
+        with pytest.raises(RuntimeError, match="not on the GPU"):
+            call()
