@@ -333,22 +333,36 @@ __global__ __launch_bounds__(64 * WM * WN * WK, resident && sizeof(T) == 2 ? 4 :
 #undef MXL_STEP
 }
 
+// the form of a product: row tiles, 32-column tiles and waves over rows, columns and channels (the kernel's parameters)
+struct MxLinForm { int rt, nj, wm, wn, wk; };
+// LDS of a workgroup that holds `chunk` steps of its rows: bytes per row, then the output staging
+struct MxLinLds { int chunk, pitch, spitch, rows, ep; };
+static MxLinLds mxl_lds(const MxLinForm& f, int S) {
+    MxLinLds l;
+    const int BM = 32 * f.rt * f.wm, EPP = 32 * f.nj + 4;
+    l.ep = (f.wk > 1 ? f.wk * 32 : 4 * 16) * EPP * 4;
+    l.chunk = S;
+    auto bytes = [&](int c) {
+        l.pitch = c * 32 + 16;                      // an odd number of 16-byte pieces: eight rows' reads hit different banks
+        l.spitch = cdiv(c, 4) * 8 + 4;
+        return BM * (l.pitch + l.spitch);
+    };
+    // all channels of the rows where they fit, else a chunk at a time
+    while ((l.rows = bytes(l.chunk)) + l.ep > 150 * 1024) l.chunk = l.chunk > 128 ? 128 : l.chunk / 2 / 4 * 4;
+    return l;
+}
+
 template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN>
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
-    constexpr int BM = 32 * RT * WM, EPP = 32 * NJ + 4;
+    constexpr int BM = 32 * RT * WM;
     constexpr int NT = 64 * WM * WN * WK;
-    const int ep = (WK > 1 ? WK * 32 : 4 * 16) * EPP * 4;
-    // LDS holds all channels of the rows where they fit, else a chunk at a time
-    int chunk = g.S;
-    auto bytes = [&](int c) {
-        g.pitch = c * 32 + 16;                      // an odd number of 16-byte pieces: eight rows' reads hit different banks
-        g.spitch = cdiv(c, 4) * 8 + 4;
-        return BM * (g.pitch + g.spitch);
-    };
-    while (bytes(chunk) + ep > 150 * 1024) chunk = chunk > 128 ? 128 : chunk / 2 / 4 * 4;
+    const MxLinLds l = mxl_lds(MxLinForm{RT, NJ, WM, WN, WK}, g.S);
+    const int chunk = l.chunk, ep = l.ep;
     g.chunk = chunk;
+    g.pitch = l.pitch;
+    g.spitch = l.spitch;
     g.sc_ofs = BM * g.pitch;
-    g.ep_ofs = (BM * (g.pitch + g.spitch) + 15) / 16 * 16;
+    g.ep_ofs = (l.rows + 15) / 16 * 16;
     const int smem = g.ep_ofs + ep;
     g.t32 = cdiv(g.N, 32);
     const int64_t mt = (g.M + BM - 1) / BM;
@@ -384,17 +398,29 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
 //   rows over the waves, 128 x 64 | 64 x 128 | 32 x 256: 65536x64x64 7.4 | 8.7 | 11.4, 65536x256x128 16.4 | 13.3 | 14.7, 65536x512x64
 //     17.5 | 17.4 | 16.4, 65536x1024x256 111 | 53 | 44
 //   32 x 256 | two row tiles, 64 x 256: 65536x256x1024 with its residual 69 | 63, 262144x64x256 52 | 41, 32768x256x512 14.4 | 15.7
+static MxLinForm mxl_form(int64_t M, int K, int N) {
+    const int64_t wgs = (M + 31) / 32 * cdiv(N, 32);
+    if (N <= 32 || wgs <= 512) return wgs <= 256 && (M < 32 ? M : 32) * K > 16384 ? MxLinForm{1, 1, 1, 1, 8} : MxLinForm{1, 1, 1, 1, 4};
+    if (N <= 64 && K <= 256) return MxLinForm{1, 2, 4, 1, 1};
+    if (N <= 128 && K <= 256) return MxLinForm{1, 2, 2, 2, 1};
+    return K <= 256 && M >= 49152 ? MxLinForm{2, 2, 1, 4, 1} : MxLinForm{1, 2, 1, 4, 1};
+}
 template <typename T, bool FULLK, bool FULLN>
 static int mxl_choose(const MxLinGeom& g, hipStream_t st) {
-    const int64_t wgs = (g.M + 31) / 32 * cdiv(g.N, 32);
-    if (g.N <= 32 || wgs <= 512) {
-        if (wgs <= 256 && (g.M < 32 ? g.M : 32) * g.K > 16384) return mxl_launch<T, 1, 1, 1, 1, 8, FULLK, FULLN>(g, st);
-        return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
-    }
-    if (g.N <= 64 && g.K <= 256) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
-    if (g.N <= 128 && g.K <= 256) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
-    if (g.K <= 256 && g.M >= 49152) return mxl_launch<T, 2, 2, 1, 4, 1, FULLK, FULLN>(g, st);
+    const MxLinForm f = mxl_form(g.M, g.K, g.N);
+    if (f.wk == 8) return mxl_launch<T, 1, 1, 1, 1, 8, FULLK, FULLN>(g, st);
+    if (f.wk == 4) return mxl_launch<T, 1, 1, 1, 1, 4, FULLK, FULLN>(g, st);
+    if (f.wm == 4) return mxl_launch<T, 1, 2, 4, 1, 1, FULLK, FULLN>(g, st);
+    if (f.wm == 2) return mxl_launch<T, 1, 2, 2, 2, 1, FULLK, FULLN>(g, st);
+    if (f.rt == 2) return mxl_launch<T, 2, 2, 1, 4, 1, FULLK, FULLN>(g, st);
     return mxl_launch<T, 1, 2, 1, 4, 1, FULLK, FULLN>(g, st);
+}
+
+extern "C" int cn_mx_linear_variant(int64_t M, int K, int N) {
+    if (M < 1 || K < 1 || N < 1 || K > MX_MAX_C || N > MX_MAX_C) return 0;
+    const MxLinForm f = mxl_form(M, K, N);
+    const int S = cdiv(K, 64);
+    return (mxl_lds(f, S).chunk < S ? 100000 : 0) + f.rt * 10000 + f.nj * 1000 + f.wm * 100 + f.wn * 10 + f.wk;
 }
 
 extern "C" int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const void* residual, void* y, int64_t M, int K, int N,

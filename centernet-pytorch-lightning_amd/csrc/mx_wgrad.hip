@@ -300,6 +300,12 @@ extern "C" size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype
     return p.splits > 1 ? sizeof(float) * (size_t)p.splits * ((size_t)N * K + N) : 0;
 }
 
+extern "C" int cn_mx_linear_wgrad_variant(int64_t rows, int K, int N, int dtype) {
+    if (rows < 1 || K < 1 || N < 1 || K > MX_MAX_C || N > MX_MAX_C) return 0;
+    const MxWgPlan p = mxwg_plan(rows, K, N, dtype);
+    return p.tn * 1000000 + p.tk * 1000 + p.splits;
+}
+
 template <typename T, int TN, int TK>
 static void mxwg_launch(const MxWgGeom& g, const MxWgPlan& p, hipStream_t st) {
     const dim3 grid(p.splits, p.ntiles * p.ktiles);

@@ -559,9 +559,14 @@ int cn_mx_pack_weight(const void* w, void* packed, int N, int K, int dtype, void
 /* y [M][N] = act(e2m1(x [M][K]) @ w4^T + bias + residual); x, residual and y in `dtype`, bias fp32 [N] */
 int cn_mx_linear_fwd(const void* x, const void* packed, const float* bias, const void* residual, void* y, int64_t M, int K, int N,
                      int relu, int dtype, void* stream);
+/* which kernel that is: RT * 10000 + NJ * 1000 + WM * 100 + WN * 10 + WK of `mx_linear_kernel<T, RT, NJ, WM, WN, WK, ...>`, + 100000 where a
+ * workgroup takes its rows' channels a chunk at a time */
+int cn_mx_linear_variant(int64_t M, int K, int N);
 /* dw [N][K] (+)= dy^T @ x8, db [N] (+)= column sums of dy (db may be null); x8 = e4m3 checkpoint [rows][K], dy [rows][N] in `dtype`.
  * Sums in a fixed order: the same inputs give the same bits. */
 size_t cn_mx_linear_wgrad_bytes(int64_t rows, int K, int N, int dtype);
+/* which kernel that is: TN * 1000000 + TK * 1000 + splits of `mx_wgrad_kernel<T, TN, TK, ...>` (a join follows where splits > 1) */
+int cn_mx_linear_wgrad_variant(int64_t rows, int K, int N, int dtype);
 int cn_mx_linear_wgrad(const void* dy, const void* codes, const void* scales, float* dw, float* db, int accumulate, int64_t rows,
                        int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream);
 /* y = act(x * scale[c] + shift[c] [+ residual]) (cn_scale_shift_act's arithmetic, any C) and x's e4m3 checkpoint in the same pass; signs (null
