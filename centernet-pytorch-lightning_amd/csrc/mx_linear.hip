@@ -356,6 +356,7 @@ template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool F
 static int mxl_launch(MxLinGeom g, hipStream_t st) {
     constexpr int BM = 32 * RT * WM;
     constexpr int NT = 64 * WM * WN * WK;
+    constexpr bool CHUNKED = RT * WM == 1;                         // (the forms of more rows are for K <= 256, which always fits)
     const MxLinLds l = mxl_lds(MxLinForm{RT, NJ, WM, WN, WK}, g.S);
     const int chunk = l.chunk, ep = l.ep;
     g.chunk = chunk;
@@ -380,13 +381,13 @@ static int mxl_launch(MxLinGeom g, hipStream_t st) {
     CN_HIP(hipGetDevice(&dev));
     if (dev >= 64 || !attr[dev]) {
         CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-        if constexpr (RT == 1)
+        if constexpr (CHUNKED)
             CN_HIP(hipFuncSetAttribute((const void*)mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         if (dev < 64) attr[dev] = true;
     }
     const dim3 grid((unsigned)mt, (unsigned)split);
-    if (RT > 1 || chunk >= g.S) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, NT, smem, st>>>(g);
-    else if constexpr (RT == 1) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, NT, smem, st>>>(g);
+    if (!CHUNKED || chunk >= g.S) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, true><<<grid, NT, smem, st>>>(g);
+    else if constexpr (CHUNKED) mx_linear_kernel<T, RT, NJ, WM, WN, WK, FULLK, FULLN, false><<<grid, NT, smem, st>>>(g);
     CN_LAUNCH_CHECK("cn_mx_linear_fwd");
     return CN_OK;
 }
