@@ -315,7 +315,7 @@ __device__ static inline float mx_stored(float v, const bf16_t*) { return bf2f(f
 
 // Forward: y = act(x scale + shift (+ residual)) and x's checkpoint in one pass (separately the checkpoint reads x and y again).  A thread
 // owns eight channels, filler included, and walks rows with its coefficients in registers; a quad of lanes is one block of 32.  Bound by
-// memory: 262144 x 256 bf16 with ReLU 75 us (345 MB, 4.6 TB/s), apply and checkpoint apart 103; 65536 x 64 8.3 | 12.0.
+// memory: 262144 x 256 bf16 with ReLU 70 us (346 MB, 4.9 TB/s), apply and checkpoint apart 103; 65536 x 64 7.3 | 12.0.
 template <typename T, bool RES, bool RELU, bool FULL>
 __global__ __launch_bounds__(256) void mx_scale_shift_act_kernel(const MxBnGeom g, const T* __restrict__ x, const T* __restrict__ res,
                                                                  const float* __restrict__ scale, const float* __restrict__ shift,

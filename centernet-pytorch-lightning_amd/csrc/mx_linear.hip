@@ -3,8 +3,11 @@
 // (v_mfma_scale_f32_32x32x64_f8f6f4: a lane's 16 bytes are one block of 32 channels, its scale rides in a byte of a register).
 //
 // What has to move is x in and y out; the codes of x never leave the workgroup.  A workgroup quantises its BM rows once into LDS and
-// keeps them there while it walks all its columns, so x is read from memory once whatever N is; the weights stream from L2 in
-// fragment order (1 KB contiguous per 32 columns x 64 channels).  K beyond what LDS holds is taken in chunks.
+// keeps them there while it walks its columns; the weights stream from L2 in fragment order (1 KB contiguous per 32 columns x 64
+// channels).  With 1024 row tiles or more a workgroup walks all columns and x is read and quantised once whatever N is (65536x1024x256:
+// 129.5 MiB read for 128 MiB of x); fewer row tiles share their columns out to as many workgroups as fill the card, and each of these reads
+// and quantises the rows again.  K beyond what LDS holds (7936 channels; 7872 and 6784 with four and eight waves over the channels) is taken in chunks, and
+// then every 256 columns (32 with waves over the channels) read and quantise x again: 4096x9000x2048 does so eight times.
 // Bound by memory: 65536x256x1024 with its residual 57 us (302 MB, 5.3 TB/s, the rate of a copy), 65536x1024x256 41 us (168 MB, 4.1 TB/s:
 // reading x alone takes 28, quantising, products and stores overlap with it in part), 1x2048x512 4.2 us (latency of one row's K).
 #include "mx_common.h"
@@ -83,6 +86,7 @@ template <int NJ> struct MxLinB { u32x4_t f[2][NJ]; };
 // 32 x 32 NJ outputs per wave; WM x WN waves over rows and columns, or WK over the channels (few rows: the launch would be short of waves
 // otherwise; their sums meet in LDS, in a fixed order).  resident: LDS holds all K channels of the rows.  RT > 1 (K <= 256): a wave takes
 // RT row tiles one after the other with the weights of its columns in registers (read from L2 half as often: 65536x256x1024 69 -> 63 us).
+// Held to four waves a SIMD (128 registers) in 16 bits, that form spills 1 - 3 of them for even K and 8 for ragged ones.
 template <typename T, int RT, int NJ, int WM, int WN, int WK, bool FULLK, bool FULLN, bool resident>
 __global__ __launch_bounds__(64 * WM * WN * WK, resident && sizeof(T) == 2 ? 4 : 2) void mx_linear_kernel(const MxLinGeom g) {
     static_assert((WK == 1 ? WM * WN == 4 : WM * WN == 1) && (RT == 1 || (WK == 1 && resident)), "rows and columns, or channels");

@@ -4,11 +4,14 @@
 // The sum runs over rows, the slow axis of both operands.  Tiles are staged in their natural [row][channel] order — the e4m3 codes
 // become bf16 on the way (exact: four significant bits times a power of two; what is below 2^-126 becomes zero) — and the transposing LDS read hands every lane eight
 // rows of its channel (rows padded by 64 B: the four rows of a read hit disjoint banks).  A 32-bit dy is split into three bf16 terms
-// (8 + 8 + 8 significant bits: nothing is lost) that share the x8 fragment.
-// Row ranges are split over workgroups; their partial sums go to the workspace and are added in a fixed order.
-// Measured: 262144x256x128 bf16 35 us + 6.5 us for the join (136 MB in: 3.9 TB/s; with the wide tiles dy and the codes are read twice and
-// once), 16384x512x2048 55 us = 0.62 PFLOP/s, where the LDS reads of a tile (768 cycles) take longer than its products (512); 1024x2048x512
-// 12.5 us, 16 row tiles in one workgroup a compute unit: latency.  32 bits: three products, 0.42 - 0.7 PFLOP/s.
+// (8 + 8 + 8 significant bits: nothing is lost from 2^-110 up; below, what lies under bf16's last 2^-133) that share the x8 fragment.
+// Row ranges are split over workgroups; their partial sums go to the workspace and are added in a fixed order.  (A join by the workgroup that
+// arrives last would save its launch, but its counters would have to live beyond the call, and two captured graphs would share them.)
+// Measured: 262144x256x128 bf16 34 us + 6.5 us for the join (136 MB in: 4.0 TB/s; both column tiles ask for dy, memory gives it once),
+// 16384x512x2048 55 us = 0.62 PFLOP/s; 1024x2048x512 13 us, 16 row tiles in one workgroup a compute unit: latency.  32 bits: three products,
+// 0.42 - 0.7 PFLOP/s (65536x1024x256 142 us).  The large sizes are bound by neither side of the loop alone: matrix pipes are busy 0.24 of
+// the time and LDS 0.30 (32 bits: 0.29 and 0.29); a tile's stages — loads' arrival, conversion, two barriers, reads, products — follow
+// one another, and two workgroups a compute unit cover that in part.
 #include "mx_common.h"
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -79,8 +82,9 @@ __global__ __launch_bounds__(256) void mx_wgrad_kernel(const MxWgGeom g) {
     constexpr int YV = BR * TN / 8 / 256, XV = BR * TK / 16 / 256;
     constexpr int YC = TN / 8, XC = TK / 16;
     constexpr int MI = TN / 64, NJ = TK / 64;                     // 2 x 2 waves of 32 x 32 tiles
-    // tiles in flight.  The wide tiles have no registers for a second; in the narrow ones it pays for 16 bits (quantising and gradient of
-    // 1024x2048x512, one | two: 18.8 | 17.4 us), not for 32 (5883x208x80 15.5 | 16.4)
+    // tiles in flight.  In the narrow ones a second pays for 16 bits (quantising and gradient of 1024x2048x512, one | two: 18.8 | 17.4 us), not
+    // for 32 (5883x208x80 15.5 | 16.4).  In the wide ones it is not measured: 16 bits take 146 of the 256 registers that their two waves a
+    // SIMD have, and a second tile 26 more
     constexpr int DEEP = sizeof(T) == 2 && TN * TK == 64 * 64 ? 2 : 1;
     constexpr int PLANE = BR * YP;
     __shared__ __attribute__((aligned(16))) bf16_t lds[NP * PLANE + BR * XP];

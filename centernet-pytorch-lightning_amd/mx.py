@@ -16,7 +16,9 @@ Work is enqueued on the current stream of the tensors' device; nothing synchroni
 call can be captured into a graph and two captured graphs share no scratch.  Results do not depend on the launch (sums have a fixed
 order).  Layers use these operators through `nn.use_checkpoints` (training) and `nn.use_mxfp4` (no-grad forward).
 
-Format.  scale = the least power of two (>= 2^-127) for which the block's largest magnitude rounds to a finite element (448 / 6);
+Format.  scale = the least power of two (>= 2^-127) for which the block's largest magnitude rounds to a finite element (448 / 6): nothing
+saturates.  (The rule that the OCP specification of these formats recommends, 2^(floor(log2 max) - emax), is half of that for the blocks
+whose largest magnitude would round past the last element, and saturates there; both decode alike.)
 value = round-to-nearest-even(x / scale) * scale, in the type asked for (next to 2^128 it may round up to an infinity).  A block that holds an infinity or a NaN stands for 32 NaNs.
 """
 import torch
@@ -253,7 +255,8 @@ def _checkpoint_of(ck, dy, what):
 def linear_wgrad(dy, ck, bias=False, into=None, bias_into=None):
     """Gradients of a linear layer / 1x1 convolution whose input was kept as `ck`: -> (dw fp32 [N, K], db fp32 [N] | None) for
     dy [..., N].  into / bias_into: contiguous fp32 tensors (of N * K / N values) the gradients are added to instead.  N and K of which
-    more than 65535 output tiles (of 64 x 64 up to 128 x 128 values) would be needed are refused."""
+    more than 65535 output tiles (of 64 x 64 up to 128 x 128 values) would be needed are refused.  Sums are 32-bit; what the checkpoint holds
+    below 2^-126 counts as zero, and of a 32-bit dy below 2^-110 what lies under 2^-133."""
     dy, dt = _tensor(dy, "mx.linear_wgrad")
     _checkpoint_of(ck, dy, "mx.linear_wgrad")
     if dy.shape[:-1] != ck.shape[:-1]:
@@ -282,7 +285,7 @@ def linear_wgrad(dy, ck, bias=False, into=None, bias_into=None):
 
 def batch_norm_act_bwd(dy, ck, gamma, mean, invstd, residual=False, racc=None, into=None):
     """Backward of y = [relu](gamma * (x - mean) * invstd + beta [+ residual]) with batch statistics over the rows, from ck =
-    mx.checkpoint(x, sign_of=y) (sign_of=None: no ReLU): -> (dx, dgamma, dbeta, dres).  residual: also return the residual input's
+    mx.checkpoint(x, sign_of=y) (sign_of=None: no ReLU; mean, invstd and the mask are the unrounded input's): -> (dx, dgamma, dbeta, dres).  residual: also return the residual input's
     gradient (racc: a tensor to add to it), else dres is None.  into: (gamma.grad, beta.grad) to add to instead of new tensors."""
     dy, dt = _tensor(dy, "mx.batch_norm_act_bwd")
     _checkpoint_of(ck, dy, "mx.batch_norm_act_bwd")

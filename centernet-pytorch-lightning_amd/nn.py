@@ -374,8 +374,10 @@ class MaxPool2d(nn.Module):
 
 def use_checkpoints(module, on=True):
     """Training with 8-bit activation checkpoints: every Conv2d and BatchNorm2d under `module` keeps its input in e4m3 (one scale per 32
-    channels) and a ReLU's mask in bits, instead of the bf16 / fp32 tensors.  The forward pass is unchanged; gradients are those of
-    the layers at the rounded inputs.  (The task heads, DCN and transposed convolutions keep what they kept, and so do the bf16 layers
+    channels) and a ReLU's mask in bits, instead of the bf16 / fp32 tensors.  The forward pass is unchanged.  A convolution's weight gradient is
+    the one at the rounded input, its other gradients are exact.  A batch norm puts the rounded input into its backward formula next to the
+    mean, variance and mask of the unrounded one, so dgamma and dx are off by that rounding, and dx sums to zero over the rows only up to it.
+    (The task heads, DCN and transposed convolutions keep what they kept, and so do the bf16 layers
     whose batch norm is applied by their consumer: they keep one tensor between the two.)  -> layers switched"""
     n = 0
     for m in module.modules():
