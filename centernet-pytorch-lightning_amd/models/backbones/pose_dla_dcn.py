@@ -196,7 +196,7 @@ class DeformConv(nn.Module):
     def forward(self, x):
         bn = self.actf[0]
         if not bn.training and not (torch.is_grad_enabled() and (self.conv.weight.requires_grad or x.requires_grad)):
-            s, b = bn.folded()
+            s, b = bn.folded(held=True)
             return self.conv.infer(x, s, b, True)
         return bn(self.conv(x, bn_stats=bn.training), None, True)
 

@@ -48,7 +48,7 @@ class PoseResNet(_MsraPoseResNet):
         for i in range(0, 18, 6):
             dcn, bn = d[i], d[i + 1]
             if not bn.training and not (torch.is_grad_enabled() and (dcn.weight.requires_grad or x.requires_grad)):
-                s, b = bn.folded()
+                s, b = bn.folded(held=True)
                 x = dcn.infer(x, s, b, True)              # eval: BN folded into the deformable conv's GEMM
             else:
                 x = bn(dcn(x), None, True)

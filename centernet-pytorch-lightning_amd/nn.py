@@ -21,24 +21,34 @@ STEM_BN_FUSED = not (os.environ.get("CN_DISABLE_STEM_BN_FUSED") or os.environ.ge
 BN_DEFER = not (os.environ.get("CN_DISABLE_BN_DEFER") or os.environ.get("CN_DISABLE_CONV_C16R") or os.environ.get("CN_DISABLE_WGRAD_C16"))
 
 
+def _capturing(device):
+    """the current stream of CUDA device index `device` (-1: the CPU) is being captured into a graph"""
+    return device >= 0 and torch._C._cuda_isCurrentStreamCapturing()
+
+
+def _state(key, a, b, c, d):
+    """what a value made from these tensors (b, c, d may be None) goes by, next to their identity"""
+    return (key, ops.WeightsEpoch.value, a._version, a.data_ptr(), None if b is None else (b._version, b.data_ptr()),
+            None if c is None else (c._version, c.data_ptr()), None if d is None else (d._version, d.data_ptr()))
+
+
 class _Entry:
     """one value of a `Derived` and what makes it safe to hand out"""
-    __slots__ = ("key", "value", "made", "memory", "tensors", "device", "stream", "done")
+    __slots__ = ("state", "value", "a", "b", "c", "d", "memory", "tensors", "device", "stream", "done")
 
-    def __init__(self, key, value, made):
-        self.key, self.value, self.made = key, value, made
+    def __init__(self, state, value, made):
+        self.state, self.value = state, value
+        self.a, self.b, self.c, self.d = made
         self.memory = [None if t is None else t.detach() for t in made]        # (the memory of `made`: no other tensor gets their addresses)
-        self.tensors = [getattr(t, "packed", t) for t in value if t is not None]
+        self.tensors = [getattr(t, "packed", t) for t in (value.values() if isinstance(value, dict) else value) if t is not None]
         self.device, self.stream, self.done = made[0].get_device(), None, None
         if self.device >= 0:
             self.stream = torch._C._cuda_getCurrentRawStream(self.device)
             self.done = torch.cuda.current_stream(self.device).record_event()
 
     def follow(self):
-        """The current stream may be another than the one that makes the value: wait for that, and let the memory not be used again before
-        this stream's work is done."""
-        if self.device < 0 or torch._C._cuda_getCurrentRawStream(self.device) == self.stream:
-            return
+        """For another stream than the one that makes the value: wait for that, and let the memory not be used again before this stream's work
+        is done."""
         here = torch.cuda.current_stream(self.device)
         if self.done is not None:
             if self.done.query():
@@ -56,12 +66,14 @@ class Derived:
 
     The replays of a graph read what its capture was given, so that stays for the layer's life (a capture at other weights keeps one more).
     What a capture itself makes exists only once the graph has run: it lies in the graph's memory and is not kept here.  (A capture does not
-    wait for the stream that made an entry: `torch.cuda.graph` has synchronised before it begins.)"""
+    wait for the stream that made an entry: `torch.cuda.graph` has synchronised before it begins.)
+
+    `find` runs for every layer of an eager forward pass, whose host time is what a small batch takes: it is written for that."""
     __slots__ = ("entry", "captured")
 
     def __init__(self):
         self.entry = None
-        self.captured = []           # entries that a captured graph reads
+        self.captured = []           # what captured graphs read: entries, tensors
 
     def __reduce__(self):
         """a copy of the layer begins anew: its parameters are others, and start at version 0 again"""
@@ -74,22 +86,25 @@ class Derived:
             d = layer.__dict__[name] = cls()
         return d
 
-    def get(self, key, made, make):
-        """make() (a tuple of tensors, packed weights or None) for `key` and the tensors `made` (the first is one, others may be None), or what
-        it gave the last time"""
-        key = (key, ops.WeightsEpoch.value, *(None if t is None else (t._version, t.data_ptr()) for t in made))
+    def find(self, key, a, b, c, d, held=False):
+        """the value kept for `key` and these tensors (b, c, d may be None), or None.  held: the caller's own entry holds the value for the graph"""
         e = self.entry
-        hit = e is not None and e.key == key and all(a is b for a, b in zip(e.made, made))
-        if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
-            if not hit:
-                return make()
-            if all(c is not e for c in self.captured):
+        if e is None or a is not e.a or b is not e.b or c is not e.c or d is not e.d or e.state != _state(key, a, b, c, d):
+            return None
+        if not held and _capturing(e.device):
+            if all(k is not e for k in self.captured):
                 self.captured.append(e)
-        elif hit:
+        elif e.device >= 0 and torch._C._cuda_getCurrentRawStream(e.device) != e.stream and not (held and _capturing(e.device)):
             e.follow()
-        else:
-            e = self.entry = _Entry(key, make(), made)
         return e.value
+
+    def keep(self, key, made, value):
+        """value (a tuple or dict of tensors, packed weights or None) is what the four tensors `made` give -> value"""
+        if _capturing(made[0].get_device()):
+            self.captured.append(made)             # (the graph makes the value again in every replay: what it reads stays)
+        else:
+            self.entry = _Entry(_state(key, *made), value, made)
+        return value
 
 
 class Conv2d(nn.Module):
@@ -143,42 +158,47 @@ class Conv2d(nn.Module):
 
     def infer_key(self, x, scale=None, shift=None):
         """-> the cache entry {wp: packed (folded) weights, b: folded bias} for x's dtype and the current parameter versions"""
-        def make():
-            wp = ops.pack_weight(self.weight, 1, x.dtype, scale)
-            b = self.bias.detach() if self.bias is not None else None
-            if shift is not None:
-                b = shift if b is None else (b * scale + shift)   # tiny [Co] host-side fold (once per weight version)
-            return wp, b
-
-        wp, b = Derived.of(self, "_packed").get(x.dtype, (self.weight, self.bias, scale, shift), make)
-        return {"wp": wp, "b": b}
+        p = self._parameters                        # (an attribute of a Module takes several times as long)
+        weight, bias = p["weight"] if "weight" in p else self.weight, p["bias"] if "bias" in p else self.bias
+        kept = Derived.of(self, "_packed")
+        hit = kept.find(x.dtype, weight, bias, scale, shift)
+        if hit is not None:
+            return hit
+        wp = ops.pack_weight(weight, 1, x.dtype, scale)
+        b = bias.detach() if bias is not None else None
+        if shift is not None:
+            b = shift if b is None else (b * scale + shift)   # tiny [Co] host-side fold (once per weight version)
+        return kept.keep(x.dtype, (weight, bias, scale, shift), {"wp": wp, "b": b})
 
     def infer(self, x, scale, shift, residual, relu, out_dtype=None):
         """No-grad path: y = act(conv(x)*scale + shift + residual); packed (folded) weights are cached."""
         if self.mx4 and out_dtype in (None, x.dtype):
             w, b = self._mx_weight(x, scale, shift)
             return mx.linear(x, w, b, residual, relu)
-        c = self.infer_key(x, scale, shift)
-        Co, _, KH, KW = self.weight.shape
+        c, p, stride, padding = self.infer_key(x, scale, shift), self._parameters, self.stride, self.padding
+        Co, _, KH, KW = (p["weight"] if "weight" in p else self.weight).shape
         N, H, W, _ = x.shape
-        OH, OW = ops.conv_out(H, KH, self.stride, self.padding), ops.conv_out(W, KW, self.stride, self.padding)
-        return ops._igemm(x, c["wp"], c["b"], residual, Co, KH, KW, self.stride, self.padding, False, relu, OH, OW, out_dtype)
+        OH, OW = ops.conv_out(H, KH, stride, padding), ops.conv_out(W, KW, stride, padding)
+        return ops._igemm(x, c["wp"], c["b"], residual, Co, KH, KW, stride, padding, False, relu, OH, OW, out_dtype)
 
     def _mx_weight(self, x, scale, shift):
         """(4-bit weights, fp32 bias) with the following BN folded in, for x's channels and this layer's padded output channels"""
-        def make():
-            Co, Ci = self.weight.shape[:2]
-            with torch.no_grad():
-                w = torch.zeros(ops.rup(Co, 16), x.shape[-1], dtype=torch.float32, device=x.device)
-                w[:Co, :Ci] = self.weight.view(Co, Ci) if scale is None else self.weight.view(Co, Ci) * scale[:, None]
-                b = torch.zeros(w.shape[0], dtype=torch.float32, device=x.device)
-                if self.bias is not None:
-                    b[:Co] = self.bias if scale is None else self.bias * scale
-                if shift is not None:
-                    b[:Co] += shift
-            return mx.pack_weight(w), b
-
-        return Derived.of(self, "_mx_cache").get((x.shape[-1], x.device), (self.weight, self.bias, scale, shift), make)
+        p = self._parameters
+        weight, bias = p["weight"] if "weight" in p else self.weight, p["bias"] if "bias" in p else self.bias
+        key, kept = (x.shape[-1], x.get_device()), Derived.of(self, "_mx_cache")
+        hit = kept.find(key, weight, bias, scale, shift)
+        if hit is not None:
+            return hit
+        Co, Ci = weight.shape[:2]
+        with torch.no_grad():
+            w = torch.zeros(ops.rup(Co, 16), x.shape[-1], dtype=torch.float32, device=x.device)
+            w[:Co, :Ci] = weight.view(Co, Ci) if scale is None else weight.view(Co, Ci) * scale[:, None]
+            b = torch.zeros(w.shape[0], dtype=torch.float32, device=x.device)
+            if bias is not None:
+                b[:Co] = bias if scale is None else bias * scale
+            if shift is not None:
+                b[:Co] += shift
+        return kept.keep(key, (weight, bias, scale, shift), (mx.pack_weight(w), b))
 
     def infer_nchw(self, x):
         """No-grad 1x1 conv + bias straight into the public fp32 NCHW layout (a head's last layer); packed weights cached as in `infer`."""
@@ -206,16 +226,20 @@ class BatchNorm2d(nn.BatchNorm2d):
             self._pending = 0
         super()._save_to_state_dict(destination, prefix, keep_vars)
 
-    def folded(self):
+    def folded(self, held=False):
         """(scale, shift) fp32 of the eval-mode affine; cached per buffer/parameter version and per `ops.WeightsEpoch` (the
-        optimizer and the training-mode kernel update parameters / running statistics behind `_version`'s back)."""
-        def make():
-            with torch.no_grad():
-                scale = self.weight * torch.rsqrt(self.running_var + self.eps)   # [C] vectors, once per weight version
-                shift = self.bias - self.running_mean * scale
-            return scale.contiguous(), shift.contiguous()
-
-        return Derived.of(self, "_folded").get(self.eps, (self.weight, self.bias, self.running_mean, self.running_var), make)
+        optimizer and the training-mode kernel update parameters / running statistics behind `_version`'s back).  held: only for a layer that
+        packs them into its own (`Derived.find`)"""
+        p, q = self._parameters, self._buffers
+        made = (p["weight"] if "weight" in p else self.weight, p["bias"] if "bias" in p else self.bias, q["running_mean"], q["running_var"])
+        kept = Derived.of(self, "_folded")
+        hit = kept.find(self.eps, *made, held)
+        if hit is not None:
+            return hit
+        with torch.no_grad():
+            scale = self.weight * torch.rsqrt(self.running_var + self.eps)   # [C] vectors, once per weight version
+            shift = self.bias - self.running_mean * scale
+        return kept.keep(self.eps, made, (scale.contiguous(), shift.contiguous()))
 
     def forward(self, x, residual=None, relu=True, defer=False):
         """defer: the caller guarantees that the ONLY consumer of the result is a 3x3 Conv2d with 16 input channels (DLA base_layer ->
@@ -251,7 +275,7 @@ def cat_conv_bn_act(conv, bn, xs, residual=None, relu=True):
     grad = torch.is_grad_enabled() and (conv.weight.requires_grad or any(t.requires_grad for t in xs))
     if bn.training or grad:
         return bn(ops.conv1x1_cat(xs, conv.weight, bn_stats=bn.training, ckpt=conv.ckpt8), residual, relu)
-    s, b = bn.folded()                              # eval: BN folded into the packed weights, one launch
+    s, b = bn.folded(held=True)                     # eval: BN folded into the packed weights, one launch
     if conv.mx4:
         return conv.infer(ops.concat(list(xs)), s, b, residual, relu)
     c = conv.infer_key(xs[0], s, b)
@@ -264,7 +288,7 @@ def conv_bn_act(conv, bn, x, residual=None, relu=True, defer=False):
         return bn(conv(x, bn_stats=True), residual, relu, defer)      # statistics from the conv kernel's epilogue where it has the hook
     if torch.is_grad_enabled() and (conv.weight.requires_grad or x.requires_grad):
         return bn(conv(x), residual, relu)          # eval-mode BN but gradients wanted: unfused affine pass
-    s, b = bn.folded()
+    s, b = bn.folded(held=True)
     return conv.infer(x, s, b, residual, relu)
 
 
@@ -349,13 +373,16 @@ class DCN(nn.Module):
 
     def infer(self, x, scale, shift, relu):
         """No-grad path with the following BN folded in: offset conv -> sampling -> ONE 1x1 GEMM (+shift, ReLU)."""
-        def make():
-            return ops.pack_weight(self.weight, 1, x.dtype, scale), (self.bias.detach() * scale + shift).contiguous()
-
-        wp, b = Derived.of(self, "_packed").get(x.dtype, (self.weight, self.bias, scale, shift), make)
+        p = self._parameters
+        weight, bias = p["weight"] if "weight" in p else self.weight, p["bias"] if "bias" in p else self.bias
+        kept = Derived.of(self, "_packed")
+        hit = kept.find(x.dtype, weight, bias, scale, shift)
+        if hit is None:
+            hit = kept.keep(x.dtype, (weight, bias, scale, shift), (ops.pack_weight(weight, 1, x.dtype, scale), (bias.detach() * scale + shift).contiguous()))
+        wp, b = hit
         N, H, W, Ci = x.shape
         om = self.conv_offset_mask.infer(x, None, None, None, False, out_dtype=torch.float32)
-        Co = self.weight.shape[0]
+        Co = weight.shape[0]
         cp = ops.rup(Co, 16)
         y = torch.empty((N, H, W, cp), dtype=x.dtype, device=x.device) if cp == Co else ops.zeros((N, H, W, cp), x.dtype, x.device)
         ops.call("cn_dcn_fwd", x, om, wp, b, y, N, H, W, Ci, Ci, Co, cp, om.shape[-1], int(relu),

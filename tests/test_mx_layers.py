@@ -27,8 +27,7 @@ def packing(lib, monkeypatch):
     """packing without a GPU: -> a dict whose "capturing" says whether the current stream is; packed weights are any bytes"""
     from centernet_amd import mx
     state = {"capturing": False}
-    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(hnn(), "_capturing", lambda device: state["capturing"])
     monkeypatch.setattr(mx, "pack_weight", lambda w: mx.MXWeight(w.reshape(-1).view(torch.uint8).clone(), *w.shape))
     return state
 
@@ -212,3 +211,20 @@ def test_inputs_that_want_a_gradient_are_refused():
     for call in (lambda: mx.quantize(xg.detach()), lambda: mx.checkpoint(xg), lambda: mx.checkpoint(x, sign_of=xg)):
         with pytest.raises(RuntimeError, match="not on the GPU"):
             call()
+
+
+def test_a_capture_that_packs_keeps_the_folded_batch_norm_it_reads(packing, monkeypatch):
+    """the batch norm was folded before the capture, the convolution is packed in it: every replay reads scale and shift again"""
+    _packs(monkeypatch)
+    monkeypatch.setattr(hnn().Conv2d, "infer", lambda self, x, s, b, res, relu: self.infer_key(x, s, b)["wp"])
+    conv, bn, x = hnn().Conv2d(4, 6, 3), hnn().BatchNorm2d(6).eval(), torch.zeros(1)
+    kept = [weakref.ref(t) for t in bn.folded()]
+    packing["capturing"] = True
+    with torch.no_grad():
+        hnn().conv_bn_act(conv, bn, x)
+    packing["capturing"] = False
+    with torch.no_grad():
+        bn.weight.add_(1)
+        hnn().conv_bn_act(conv, bn, x)
+    gc.collect()
+    assert all(r() is not None for r in kept)
