@@ -1107,7 +1107,8 @@ class BatchNormCkptFn(Function):
                  stats[2:], npix, C, BN_MOMENTUM, BN_EPS)
             BnStats.release(part)                 # handed back all-zero
         else:
-            ws, n = _bn_ws(npix, C, x.device)
+            n = _hip.query("cn_bn_workspace_bytes", npix, C)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)            # (not the stream's: two captured graphs would share that)
             call("cn_bn_train_stats", x, gamma.detach(), beta.detach(), running_mean, running_var, stats[0], stats[1], stats[2:], npix, C,
                  BN_MOMENTUM, BN_EPS, dtype_code(x.dtype), ws, n)
         y, ck = mx.scale_shift_act(x, stats[2], stats[3], residual, relu)

@@ -230,3 +230,41 @@ def test_biases_of_a_head_train_above_frozen_weights(rows):
     assert got[True][0] is None and got[True][2] is None
     for i in (1, 3):
         assert got[True][i] is not None and torch.allclose(got[True][i], got[False][i], rtol=1e-4, atol=1e-4 * float(got[False][i].abs().max()))
+
+
+def test_graphs_of_checkpointed_batch_norms_side_by_side(monkeypatch):
+    """two layers' forward and backward passes, captured on one stream, replayed at once on two: they share no scratch"""
+    n = hnn()
+    bns = [n.BatchNorm2d(96).to(DEV).train() for _ in range(2)]
+    xs = [img((4, 40, 40, 96), 1 + i, F32, 2.0 ** i) for i in range(2)]
+    dys = [img((4, 40, 40, 96), 5 + i, F32, 1e-2) for i in range(2)]
+
+    def step(i):
+        xi = xs[i].detach().requires_grad_()
+        y = bns[i](xi, None, True)
+        return (y.detach(), *torch.autograd.grad(y, (xi, bns[i].weight, bns[i].bias), dys[i]))
+
+    for bn in bns:
+        n.use_checkpoints(bn)
+    wants = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    from centernet_amd import _hip
+    monkeypatch.setattr(_hip, "workspace", None)                   # the stream's own scratch is not asked for
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(i))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(6):
+        for o in outs:
+            for t in o:
+                t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, wants):
+            assert all(torch.equal(a, b) for a, b in zip(o, w)), rep
