@@ -34,29 +34,26 @@ def _state(key, a, b, c, d):
 
 class _Entry:
     """one value of a `Derived` and what makes it safe to hand out"""
-    __slots__ = ("state", "value", "a", "b", "c", "d", "memory", "tensors", "device", "stream", "done")
+    __slots__ = ("state", "value", "a", "b", "c", "d", "memory", "tensors", "device", "streams", "done")
 
     def __init__(self, state, value, made):
         self.state, self.value = state, value
         self.a, self.b, self.c, self.d = made
         self.memory = [None if t is None else t.detach() for t in made]        # (the memory of `made`: no other tensor gets their addresses)
         self.tensors = [getattr(t, "packed", t) for t in (value.values() if isinstance(value, dict) else value) if t is not None]
-        self.device, self.stream, self.done = made[0].get_device(), None, None
+        self.device = made[0].get_device()
         if self.device >= 0:
-            self.stream = torch._C._cuda_getCurrentRawStream(self.device)
+            self.streams = {torch._C._cuda_getCurrentRawStream(self.device)}       # that may use the value as it is
             self.done = torch.cuda.current_stream(self.device).record_event()
 
     def follow(self):
-        """For another stream than the one that makes the value: wait for that, and let the memory not be used again before this stream's work
-        is done."""
+        """The first call on another stream than the one that makes the value: what this stream does from now on waits for that, and the memory is
+        not given away before this stream is done with it."""
         here = torch.cuda.current_stream(self.device)
-        if self.done is not None:
-            if self.done.query():
-                self.done = None
-            else:
-                here.wait_event(self.done)
+        here.wait_event(self.done)
         for t in self.tensors:
             t.record_stream(here)
+        self.streams.add(here.cuda_stream)
 
 
 class Derived:
@@ -94,7 +91,7 @@ class Derived:
         if not held and _capturing(e.device):
             if all(k is not e for k in self.captured):
                 self.captured.append(e)
-        elif e.device >= 0 and torch._C._cuda_getCurrentRawStream(e.device) != e.stream and not (held and _capturing(e.device)):
+        elif e.device >= 0 and torch._C._cuda_getCurrentRawStream(e.device) not in e.streams and not (held and _capturing(e.device)):
             e.follow()
         return e.value
 
