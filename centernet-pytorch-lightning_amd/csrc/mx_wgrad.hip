@@ -279,6 +279,8 @@ __global__ __launch_bounds__(256) void mx_wgrad_join_kernel(const float* __restr
 // us, wide | narrow, bf16: 262144x256x128 43 | 56, 65536x1024x256 53 | 72, 16384x512x2048 56 | 74, 25394x224x660 31 | 46;
 // 8192x512x512 24.3 | 21.8, 65536x256x64 18.5 | 15.2, 4096x1024x256 19.1 | 16.5, 1024x2048x512 18.3 | 12.4 (15.8 in two splits),
 // 204x800x732 7.4 (10.6 in two splits), 15993x22x51 10.9 (13.2 with a row tile a split).
+// The border goes by products alone.  Below it, gradient alone, wide | narrow: 131072x128x128 22.8 | 19.7, 65536x256x128 21.1 | 18.8, 16384x256x512
+// 20.1 | 19.2, 2048x1024x1024 26.5 | 21.0; only many rows of one tile would be better off wide: 262144x128x80 23.7 | 26.7, 262144x80x80 21.9 | 25.9.
 // 32 bits (64 x 128 | 64 x 64): 65536x1024x256 137 | 176, 65536x256x64 20.4 | 22.7, 30000x80x208 20.2 | 24.0; 831x864x560 17.1 | 16.2.
 struct MxWgPlan { bool wide; int tn, tk, ntiles, ktiles, splits; int64_t per; };
 static MxWgPlan mxwg_plan(int64_t rows, int K, int N, int dtype) {
